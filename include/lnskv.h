@@ -276,6 +276,100 @@ int lnskv_prefill_attention(const lnskv_pages* c, const float* q_dev, float* out
                             lnskv_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Rotary positions of several axes (time, height and width of pictures and
+ * video).  The reference turns every pair of a head by one position
+ * (lns_decode.metal:154-191); here pair i (dims i and i + rotary_dim/2) turns by
+ * the position of the axis it belongs to:
+ *   angle_i = axis_pos[axis(i)][t] * inv_freqs[i]   (an f64 product; sine and
+ *   cosine rounded once to f32, so far positions lose nothing; the one-position
+ *   entry points above round the angle itself to f32, as the reference does)
+ * sections (host, [n_axes], n_axes 1..4, summing to rotary_dim/2) gives each axis
+ * its number of pairs: interleaved 0: the first sections[0] pairs are axis 0's,
+ * the next sections[1] axis 1's, ...; interleaved 1: pairs are dealt in turn,
+ * axis(i) = i % n_axes while i < n_axes * sections[i % n_axes], axis 0 after
+ * (sections that cannot be dealt so are refused).
+ * lnskv_mrope_append stores token t's K (every kv head turned) and V in the slot
+ * of tok_pos_dev[t] of table row tok_seq_dev[t] as lnskv_append does, skipping
+ * the same tokens, and writes q_dev [n_tok][n_heads][head_dim], turned by the
+ * same positions, to q_out_dev (q_dev itself or a buffer apart from it; both
+ * NULL: no queries, n_heads is not read).  One kernel for prompts and for single
+ * tokens: tok_pos is where a token is stored, axis_pos_dev [n_axes][n_tok] (any
+ * int32) what it turns by.  k_new_dev, v_new_dev and q_dev are left as they are
+ * (q_out_dev == q_dev apart).  No two tokens of a call may share a slot.
+ * ------------------------------------------------------------------------- */
+int lnskv_mrope_append(const lnskv_pages* c, const lnskv_rope* rope, const int32_t* sections,
+                       int32_t n_axes, int32_t interleaved, const float* q_dev, float* q_out_dev,
+                       int32_t n_heads, const float* k_new_dev, const float* v_new_dev,
+                       const int32_t* axis_pos_dev, const int32_t* tok_seq_dev,
+                       const int32_t* tok_pos_dev, int32_t n_tok, const uint32_t* block_tables_dev,
+                       int32_t bt_stride, int32_t n_rows, lnskv_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Sliding window with sinks: the first n_sink tokens of a sequence stay visible
+ * behind its window.  The reference has the window alone (kv_p_start, engine.rs:
+ * 3007-3013).  A query at position p attends the tokens t <= p with t < n_sink or
+ * t > p - window (window = 0: every t <= p), each once.  Pages that hold
+ * neither are not looked at: their table entries may be anything
+ * (lnskv_evict_kv_pages_sink frees them).
+ * lnskv_sink_decode: lnskv_decode with this rule, the query of sequence s at
+ * position kv_len_dev[s] - 1 (append its token first); gate_dev (NULL: none) as in
+ * lnskv_gated_append_decode; workspace as lnskv_decode's, of
+ * lnskv_sink_decode_workspace_size bytes (same n_seq, n_heads, max_kv_len, window
+ * and n_sink, same current device) or NULL.  Every page type and shape of
+ * lnskv_decode; n_sink in [0, 2^30].
+ * lnskv_sink_prefill_attention: lnskv_prefill_attention with this rule (f16 or
+ * Q8A pages, head_dim 128 or 256).
+ * ------------------------------------------------------------------------- */
+int lnskv_sink_decode_workspace_size(const lnskv_pages* c, int32_t n_seq, int32_t n_heads,
+                                     int32_t max_kv_len, int32_t window, int32_t n_sink, size_t* bytes);
+int lnskv_sink_decode(const lnskv_pages* c, const float* q_dev, float* out_dev, const float* gate_dev,
+                      const uint32_t* block_tables_dev, int32_t bt_stride, const int32_t* kv_len_dev,
+                      int32_t n_seq, int32_t n_heads, int32_t max_kv_len, int32_t window,
+                      int32_t n_sink, float scale, void* workspace_dev, size_t ws_bytes,
+                      lnskv_stream_t stream);
+int lnskv_sink_prefill_attention(const lnskv_pages* c, const float* q_dev, float* out_dev,
+                                 const int32_t* chunks_dev, int32_t n_chunks, int32_t n_tok,
+                                 const uint32_t* block_tables_dev, int32_t bt_stride, int32_t n_rows,
+                                 int32_t window, int32_t n_sink, int32_t n_heads, float scale,
+                                 lnskv_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Shared prefixes: lnskv_decode for a batch in which runs of sequences begin
+ * with the same pages (lnskv_fork_sequence makes them).  The pages of a group
+ * are read once for all its query rows instead of once per sequence.  The
+ * reference decodes one sequence (engine.rs:1442-1448).
+ *   groups: host array [n_groups][3] of {first sequence, sequences, shared
+ *   tokens}, read before the call returns: runs of sequences in ascending order,
+ *   none in two groups; at most LNSKV_PREFIX_MAX_GROUPS.  The first shared tokens
+ *   / 16 (rounded down) pages of every sequence of a group are taken from table
+ *   row `first sequence`; the other rows' entries for them are not read.
+ *   Sequences outside every group are decoded by themselves.
+ *   Everything else as lnskv_decode with p_start = 0 and split_tokens = 0: sequence s
+ *   attends [0, kv_len_dev[s]), also where that ends inside the shared pages; a
+ *   length out of range gives a zero row.  Append the newest tokens first, into
+ *   pages that are not shared.  gate_dev (NULL: none) as in
+ *   lnskv_gated_append_decode.  workspace_dev / ws_bytes:
+ *   lnskv_prefix_decode_workspace_size bytes (same groups, shape and current
+ *   device) or NULL, with lnskv_decode's rules.  Under graph capture the groups
+ *   are the captured call's.
+ * lnskv_shared_prefix_groups (host) finds the groups of rows [0, n_seq): from row
+ *   r on, the rows that share at least min_pages (>= 1) leading pages with row r
+ *   form a group whose shared tokens are 16 * the pages that all of them share, at
+ *   most LNSKV_PREFIX_MAX_GROUPS of them.  groups receives *n_groups rows of 3.  A
+ *   page counts as shared only where it is allocated and is not the last of a row
+ *   (that one may still be written).
+ * ------------------------------------------------------------------------- */
+#define LNSKV_PREFIX_MAX_GROUPS 128
+int lnskv_prefix_decode_workspace_size(const lnskv_pages* c, const int32_t* groups, int32_t n_groups,
+                                       int32_t n_seq, int32_t n_heads, int32_t max_kv_len,
+                                       size_t* bytes);
+int lnskv_prefix_decode(const lnskv_pages* c, const float* q_dev, float* out_dev, const float* gate_dev,
+                        const uint32_t* block_tables_dev, int32_t bt_stride, const int32_t* kv_len_dev,
+                        const int32_t* groups, int32_t n_groups, int32_t n_seq, int32_t n_heads,
+                        int32_t max_kv_len, float scale, void* workspace_dev, size_t ws_bytes,
+                        lnskv_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Gated attention (gated_query_attention models): the q projection holds, per
  * query head, head_dim q values then head_dim gate logits; the attention
  * output is multiplied by sigmoid(logits) before o_proj.
@@ -476,6 +570,19 @@ int lnskv_step_pages(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t layer
  * consecutive positions touches, (window + 14) / 16 + 1.  0 for window <= 0
  * (full attention: the context length decides). */
 int32_t lnskv_window_pages(int32_t window);
+/* The same for a window behind n_sink sinks (lnskv_sink_decode): pages that hold
+ * one of the first n_sink tokens stay.  lnskv_evict_kv_pages_sink frees the other
+ * pages wholly before the window; lnskv_step_pages_sink does so and then ensures
+ * position pos; lnskv_sink_window_pages is what a pool needs per sequence for that:
+ * lnskv_window_pages(window) + ceil(n_sink / 16), 0 for window <= 0. */
+int lnskv_evict_kv_pages_sink(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t seq,
+                              int32_t pos, int32_t window, int32_t n_sink);
+int lnskv_step_pages_sink(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t layer, int32_t seq,
+                          int32_t pos, int32_t window, int32_t n_sink);
+int32_t lnskv_sink_window_pages(int32_t window, int32_t n_sink);
+/* Groups of rows that share their leading pages, for lnskv_prefix_decode. */
+int lnskv_shared_prefix_groups(const lnskv_block_tables* t, int32_t n_seq, int32_t min_pages,
+                               int32_t* groups, int32_t* n_groups);
 /* Free every page of row seq (sequence finished or evicted) and empty it. */
 int lnskv_free_sequence(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t seq);
 /* Copy-on-write fork: row child becomes a view of the first n_tok tokens of

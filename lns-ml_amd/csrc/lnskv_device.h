@@ -141,8 +141,8 @@ __device__ __forceinline__ float cross_max(float x) {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// RoPE's sine and cosine of the f32 angle theta (pos * inv_freq, the
-// reference's angle), each rounded once to f32 from an f64 evaluation:
+// Sine and cosine of the f64 angle t; rope_sincos: RoPE's of the f32 angle
+// theta (pos * inv_freq, the reference's angle).  Each rounded once to f32 from an f64 evaluation:
 // Cody-Waite reduction by pi/2 (pi/2 split into two 26-bit parts and a 53-bit
 // tail, so that k times a part is exact for |k| < 2^27), then Taylor
 // polynomials in r^2 on |r| <= pi/4 (sine to r^17, cosine to r^18:
@@ -151,9 +151,8 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 // rotated values agree bit for bit; both equal the correctly rounded sin/cos
 // unless the exact value lies within ~1e-16 (relative) of an f32 rounding
 // boundary.
-__device__ __forceinline__ void rope_sincos(float theta, float* s, float* c) {
+__device__ __forceinline__ void rope_sincos_f64(double t, float* s, float* c) {
 #pragma clang fp contract(off)
-  const double t = (double)theta;
   const double k = rint(t * 0x1.45f306dc9c883p-1);  // nearest multiple of pi/2
   const double r = ((t - k * 0x1.921fb5p+0) - k * 0x1.110b46p-26) - k * 0x1.1a62633145c07p-54;
   const double z = r * r;
@@ -182,6 +181,7 @@ __device__ __forceinline__ void rope_sincos(float theta, float* s, float* c) {
   *s = (float)sv;
   *c = (float)cv;
 }
+__device__ __forceinline__ void rope_sincos(float theta, float* s, float* c) { rope_sincos_f64((double)theta, s, c); }
 
 // One RoPE pair (x0, x1) = (dim i, dim i + half) turned by (s, c): x0 c - x1 s
 // and x0 s + x1 c, each product and each sum rounded once (no fused
@@ -256,6 +256,75 @@ __device__ __forceinline__ float gated(const DecodeArgs& a, size_t idx, float v)
   return a.gate ? v * a.gate[idx] : v;
 }
 
+// ---------------------------------------------------------------------------
+// Which tokens a decode kernel attends for a sequence of length L:
+//  kPlain   [p_start, L)
+//  kSink    the first n_sink tokens and the last `window` (0: all of them)
+//  kPrefix  [P, L), P the tokens that the sequence shares with its group; what
+//           the group's prefix gives its rows comes as a partial row per query
+//           head (numerator, running max, sum), merged where the segment's
+//           first page is
+enum DecodeVariant { kPlain = 0, kSink = 1, kPrefix = 2 };
+template <int VAR> struct VarArgs {};
+template <> struct VarArgs<kSink> {
+  int32_t window;
+  int32_t n_sink;
+};
+// Sequences [first, end) share their first `pages` pages, held by row `first`.
+struct PrefixGroup {
+  int32_t first, end, pages;
+};
+template <> struct VarArgs<kPrefix> {
+  const float* seed_acc;  // [n_seq][n_heads][D] numerators of the prefix
+  const float* seed_ml;   // [n_seq][n_heads][2] running max (log2 units) and sum
+  int32_t s0;             // the launch's first sequence
+  int32_t n_groups;
+  PrefixGroup g[LNSKV_PREFIX_MAX_GROUPS];
+};
+
+// Shared pages of the launch's sequence s; 0 where it is in no group.
+__device__ __forceinline__ int shared_pages(const VarArgs<kPrefix>& x, int s) {
+  int p = 0;
+  for (int i = 0; i < x.n_groups; ++i)
+    if (s + x.s0 >= x.g[i].first && s + x.s0 < x.g[i].end) p = x.g[i].pages;
+  return p;
+}
+
+// kSink: the attended tokens of a sequence are t < n_sink and p0 <= t < L.
+// Its pages are numbered without the `gap` pages between the sinks' and the
+// window's: page v is table entry v for v < sinkp, v + gap after.
+struct SinkSpan {
+  int L, p0, n_sink, sinkp, gap;
+};
+__device__ __forceinline__ SinkSpan sink_span(const VarArgs<kSink>& x, int L) {
+  SinkSpan v;
+  v.L = L;
+  v.p0 = x.window > 0 ? max(L - x.window, 0) : 0;
+  v.n_sink = x.n_sink;
+  v.sinkp = (x.n_sink + kPage - 1) / kPage;
+  v.gap = max(v.p0 / kPage - v.sinkp, 0);
+  return v;
+}
+__device__ __forceinline__ int sink_entry(const SinkSpan& sp, int v) { return v < sp.sinkp ? v : v + sp.gap; }
+// Whether token t is attended, and whether the 16 tokens from t on all are.
+__device__ __forceinline__ bool sink_sees(const SinkSpan& sp, int t) { return t < sp.L && (t >= sp.p0 || t < sp.n_sink); }
+__device__ __forceinline__ bool sink_sees_page(const SinkSpan& sp, int t) {
+  return t + kPage <= sp.L && (t >= sp.p0 || t + kPage <= sp.n_sink);
+}
+__device__ __forceinline__ bool span_sees(int t, const SinkSpan& sp) { return sink_sees(sp, t); }
+__device__ __forceinline__ bool span_sees(int) { return true; }
+// The kernels pass what belongs to a variant as a parameter pack that is empty
+// for kPlain, so that the plain kernels compile to what they are without it:
+// the arguments of a call (VarArgs), the span of a sequence (SinkSpan), the
+// seed rows of a piece (PieceSeed).
+template <class X>
+__device__ __forceinline__ const X& only(const X& x) { return x; }
+struct PieceSeed {  // kPrefix: the rows that the piece which starts a segment merges
+  bool seeded;
+  const float* acc;
+  const float* ml;
+};
+
 struct SeqWindow {
   int L;       // kv_len; 0 when it is past what the grid or the table row can address
   int p0;      // window start
@@ -263,14 +332,24 @@ struct SeqWindow {
   int nparts;  // partitions of this sequence
 };
 
-template <bool FUSED>
-__device__ __forceinline__ SeqWindow seq_window(const DecodeArgs& a, int s) {
+template <bool FUSED, int VAR = kPlain, class... X>
+__device__ __forceinline__ SeqWindow seq_window(const DecodeArgs& a, int s, const X&... x) {
   SeqWindow w;
   int L = a.kv_len ? a.kv_len[s] : a.kv_len_scalar;
   // a length past what the grid or the table row can address marks the
   // sequence out of range: empty window, nothing stored
   L = L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : max(L, 0);
+  if constexpr (VAR == kSink) {  // partitions of the pages without the gap
+    const SinkSpan sp = sink_span(only(x...), L);
+    w.L = L;
+    w.p0 = 0;
+    w.jf = 0;
+    const int np = L > 0 ? (L - 1) / kPage + 1 - sp.gap : 0;
+    w.nparts = max(1, (np * kPage + a.split - 1) / a.split);
+    return w;
+  }
   int p0 = a.p_start ? a.p_start[s] : a.p_start_scalar;
+  if constexpr (VAR == kPrefix) p0 = shared_pages(only(x...), s) * kPage;
   p0 = min(max(p0, 0), L);
   int lo = p0;
   if (FUSED && L > 0) lo = min(lo, L - 1);
@@ -304,9 +383,10 @@ struct EpilogueLds {
   float l[kWavesPerBlock][REP];
 };
 
-template <int REP, int D>
+// kPrefix: the first partition's block merges the prefix's row as well.
+template <int REP, int D, int VAR = kPlain, class... X>
 __device__ __forceinline__ void finish_block(const DecodeArgs& a, EpilogueLds<REP, D>& sm, const SeqWindow& w,
-                                             int s, int kvh, int part) {
+                                             int s, int kvh, int part, const X&... x) {
   const int h0 = kvh * REP;
   const bool single = w.nparts == 1;
   for (int idx = threadIdx.x; idx < REP * D; idx += kBlock) {
@@ -322,6 +402,16 @@ __device__ __forceinline__ void finish_block(const DecodeArgs& a, EpilogueLds<RE
       Ls = fmaf(wq, sm.l[q][h], Ls);
     }
     const size_t hrow = (size_t)s * a.n_heads + h0 + h;
+    if constexpr (VAR == kPrefix) {
+      if (part == 0 && w.p0 > 0) {  // block-uniform
+        const VarArgs<kPrefix>& pf = only(x...);
+        const float ms = pf.seed_ml[2 * hrow], Mn = fmaxf(M, ms);
+        const float wa = fast_exp2(M - Mn), wb = fast_exp2(ms - Mn);
+        A = A * wa + pf.seed_acc[hrow * D + i] * wb;
+        Ls = Ls * wa + pf.seed_ml[2 * hrow + 1] * wb;
+        M = Mn;
+      }
+    }
     if (single) {
       a.out[hrow * D + i] = gated(a, hrow * D + i, Ls > 0.0f ? A / Ls : 0.0f);
     } else {
@@ -418,10 +508,10 @@ __device__ __forceinline__ void merge_partials(const float2* ml, const float* ac
   }
 }
 
-template <int REP, int D, bool FUSED>
-__global__ __launch_bounds__(kBlock) void combine_kernel(DecodeArgs a) {
+template <int REP, int D, bool FUSED, int VAR = kPlain, class... X>
+__global__ __launch_bounds__(kBlock) void combine_kernel(DecodeArgs a, X... x) {
   const int kvh = blockIdx.x, s = blockIdx.y, h = blockIdx.z;
-  const SeqWindow w = seq_window<FUSED>(a, s);
+  const SeqWindow w = seq_window<FUSED, VAR>(a, s, x...);
   if (w.nparts <= 1) return;  // block-uniform: the decode kernel wrote the output
   const int np = min(w.nparts, a.max_parts);
   const size_t hrow = (size_t)s * a.n_heads + (size_t)kvh * REP + h;
@@ -431,10 +521,10 @@ __global__ __launch_bounds__(kBlock) void combine_kernel(DecodeArgs a) {
                     a.gate ? a.gate + hrow * D : nullptr);
 }
 
-template <int REP, int D, bool FUSED>
-inline void launch_combine(const DecodeArgs& a, int n_seq, hipStream_t st) {
+template <int REP, int D, bool FUSED, int VAR = kPlain, class... X>
+inline void launch_combine(const DecodeArgs& a, int n_seq, hipStream_t st, const X&... x) {
   if (a.max_parts > 1)
-    combine_kernel<REP, D, FUSED><<<dim3((unsigned)a.n_kv, (unsigned)n_seq, REP), kBlock, 0, st>>>(a);
+    combine_kernel<REP, D, FUSED, VAR><<<dim3((unsigned)a.n_kv, (unsigned)n_seq, REP), kBlock, 0, st>>>(a, x...);
 }
 
 // Launchers (defined in the decode translation units).
@@ -479,12 +569,19 @@ struct PrefillArgs {
   int32_t n_heads;
   uint32_t num_pages;
   float scale_log2;
+  int32_t n_sink;          // launch_prefill_mfma_sink: tokens t < n_sink are attended too
 };
 // Queries per tile of the prefill kernel (a workgroup per tile and kv head).
 int prefill_queries_per_tile(int rep, int head_dim);
 int launch_prefill_mfma(const PrefillArgs& a, int rep, int head_dim, int n_tiles, hipStream_t st);
+int launch_prefill_mfma_sink(const PrefillArgs& a, int rep, int head_dim, int n_tiles, hipStream_t st);
 
 int hip_check(const char* what);
+// Tokens per split-K partition when the caller leaves it to the library, and
+// the schedule that LNSKV_DECODE_SCHEDULE asks for.
+int choose_split(int n_seq, int n_kv, int max_kv_len);
+enum { kScheduleAuto = 0, kScheduleStreamK = 1, kScheduleWorkgroup = 2 };
+int schedule_setting();
 // A device buffer the library keeps per device: 0 the decode workspace, 1
 // RoPE'd q/k rows, 2 the Q4L GEMV's partial sums.  Growing it allocates a new
 // buffer and keeps the old one until lnskv_workspace_release (no device

@@ -328,6 +328,71 @@ int lnskv_step_pages(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t layer
   return lnskv_ensure_kv_page(t, pool, layer, seq, pos);
 }
 
+int lnskv_evict_kv_pages_sink(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t seq, int32_t pos,
+                              int32_t window, int32_t n_sink) {
+  if (!row_ok(t, seq) || !pool) return fail(LNSKV_ERR_INVALID, "bad table/pool or seq %d", seq);
+  if (n_sink < 0) return fail(LNSKV_ERR_INVALID, "n_sink %d is negative", n_sink);
+  if (window <= 0) return LNSKV_OK;
+  const int32_t evict_before = lnskv_kv_p_start(pos, window) / LNSKV_PAGE_SIZE;
+  const int32_t kept = (int32_t)(((int64_t)n_sink + LNSKV_PAGE_SIZE - 1) / LNSKV_PAGE_SIZE);
+  uint32_t* row = t->table.data() + (size_t)seq * (size_t)t->max_pages;
+  const int32_t n = std::min(evict_before, t->len[(size_t)seq]);
+  for (int32_t lp = kept; lp < n; ++lp) {
+    if (row[lp] != LNSKV_NO_PAGE) {
+      if (int rc = lnskv_page_pool_free(pool, row[lp])) return rc;
+      set_entry(t, seq, lp, LNSKV_NO_PAGE);
+    }
+  }
+  return LNSKV_OK;
+}
+
+int lnskv_step_pages_sink(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t layer, int32_t seq, int32_t pos,
+                          int32_t window, int32_t n_sink) {
+  if (int rc = lnskv_evict_kv_pages_sink(t, pool, seq, pos, window, n_sink)) return rc;
+  return lnskv_ensure_kv_page(t, pool, layer, seq, pos);
+}
+
+int32_t lnskv_sink_window_pages(int32_t window, int32_t n_sink) {
+  if (window <= 0) return 0;
+  return (int32_t)(lnskv_window_pages(window) + ((int64_t)std::max(n_sink, 0) + LNSKV_PAGE_SIZE - 1) / LNSKV_PAGE_SIZE);
+}
+
+int lnskv_shared_prefix_groups(const lnskv_block_tables* t, int32_t n_seq, int32_t min_pages, int32_t* groups,
+                               int32_t* n_groups) {
+  if (!t || !groups || !n_groups) return fail(LNSKV_ERR_INVALID, "table, groups and n_groups must be non-null");
+  *n_groups = 0;
+  if (n_seq < 0 || n_seq > t->n_seq) return fail(LNSKV_ERR_INVALID, "n_seq %d out of range [0, %d]", n_seq, t->n_seq);
+  if (min_pages < 1) return fail(LNSKV_ERR_INVALID, "min_pages %d must be at least 1", min_pages);
+  // leading pages that rows a and b share, their last pages apart
+  auto shared = [&](int32_t a, int32_t b) {
+    const uint32_t* ra = t->table.data() + (size_t)a * (size_t)t->max_pages;
+    const uint32_t* rb = t->table.data() + (size_t)b * (size_t)t->max_pages;
+    const int32_t most = std::min(t->len[(size_t)a], t->len[(size_t)b]) - 1;
+    int32_t k = 0;
+    while (k < most && ra[k] != LNSKV_NO_PAGE && ra[k] == rb[k]) ++k;
+    return k;
+  };
+  int32_t n = 0;
+  for (int32_t r = 0; r + 1 < n_seq && n < LNSKV_PREFIX_MAX_GROUPS;) {
+    int32_t end = r + 1, pages = t->len[(size_t)r];
+    while (end < n_seq) {
+      const int32_t k = shared(r, end);
+      if (k < min_pages) break;
+      pages = std::min(pages, k);
+      ++end;
+    }
+    if (end - r > 1) {
+      groups[3 * n] = r;
+      groups[3 * n + 1] = end - r;
+      groups[3 * n + 2] = pages * LNSKV_PAGE_SIZE;
+      ++n;
+    }
+    r = end;
+  }
+  *n_groups = n;
+  return LNSKV_OK;
+}
+
 int lnskv_free_sequence(lnskv_block_tables* t, lnskv_page_pool* pool, int32_t seq) {
   if (!row_ok(t, seq) || !pool) return fail(LNSKV_ERR_INVALID, "bad table/pool or seq %d", seq);
   uint32_t* row = t->table.data() + (size_t)seq * (size_t)t->max_pages;

@@ -59,6 +59,28 @@ uint32_t* ws_error_word(void* stream, bool allocate) {
   return w;
 }
 
+// Tokens per split-K partition when the caller passes 0: the largest power
+// of two in [64, 1024] that still gives about 1024 workgroups (4 per CU) if
+// sequences average half of max_kv_len.
+int choose_split(int n_seq, int n_kv, int max_kv_len) {
+  const int64_t pairs = (int64_t)n_seq * n_kv;
+  int split = 1024;
+  while (split > 64 && pairs * max_kv_len < (int64_t)2 * split * 1024) split /= 2;
+  return split;
+}
+
+// LNSKV_DECODE_SCHEDULE=stream-k or =workgroup forces that schedule wherever
+// the library would choose between the two (tests, tuning); unset or any
+// other value: by batch size.  Read on every plan, so that a workspace query
+// and the call it sizes see the same setting.
+int schedule_setting() {
+  const char* v = std::getenv("LNSKV_DECODE_SCHEDULE");
+  if (v == nullptr) return kScheduleAuto;
+  if (std::strcmp(v, "stream-k") == 0) return kScheduleStreamK;
+  if (std::strcmp(v, "workgroup") == 0) return kScheduleWorkgroup;
+  return kScheduleAuto;
+}
+
 int take_ws_error() {
   uint32_t* w = g_ws_err.load(std::memory_order_acquire);
   return w ? (int)__atomic_exchange_n(w, 0u, __ATOMIC_ACQ_REL) : 0;
@@ -371,15 +393,6 @@ int launch_decode(const DecodeArgs& a, int dtype, int d, int rep, int n_seq, hip
   }
 }
 
-// Tokens per split-K partition when the caller passes 0: the largest power
-// of two in [64, 1024] that still gives about 1024 workgroups (4 per CU) if
-// sequences average half of max_kv_len.
-int choose_split(int n_seq, int n_kv, int max_kv_len) {
-  const int64_t pairs = (int64_t)n_seq * n_kv;
-  int split = 1024;
-  while (split > 64 && pairs * max_kv_len < (int64_t)2 * split * 1024) split /= 2;
-  return split;
-}
 
 // Workspace (only needed when some sequence spans several split-K
 // partitions): partial numerators [n_seq][n_heads][max_parts][d] f32, then
@@ -452,18 +465,6 @@ struct DecodePlan {
   size_t ws_bytes = 0;
 };
 
-// LNSKV_DECODE_SCHEDULE=stream-k or =workgroup forces that schedule wherever
-// the library would choose between the two (tests, tuning); unset or any
-// other value: by batch size.  Read on every plan, so that a workspace query
-// and the call it sizes see the same setting.
-enum { kScheduleAuto = 0, kScheduleStreamK = 1, kScheduleWorkgroup = 2 };
-int schedule_setting() {
-  const char* v = std::getenv("LNSKV_DECODE_SCHEDULE");
-  if (v == nullptr) return kScheduleAuto;
-  if (std::strcmp(v, "stream-k") == 0) return kScheduleStreamK;
-  if (std::strcmp(v, "workgroup") == 0) return kScheduleWorkgroup;
-  return kScheduleAuto;
-}
 
 int plan_decode(const lnskv_pages* c, int n_seq, int n_heads, int max_kv_len, int split_tokens, int fused,
                 DecodePlan* p) {
@@ -1093,10 +1094,12 @@ int lnskv_gated_append_decode(const lnskv_pages* c, const lnskv_rope* rope, cons
                             n_heads, max_kv_len, scale, split_tokens, ws, ws_bytes, stream, rope, gate);
 }
 
-int lnskv_prefill_attention(const lnskv_pages* c, const float* q, float* out, const int32_t* chunks,
-                            int32_t n_chunks, int32_t n_tok, const uint32_t* bt, int32_t bt_stride, int32_t n_rows,
-                            const int32_t* p_start, int32_t window, int32_t n_heads, float scale,
-                            lnskv_stream_t stream) {
+namespace lnskv {
+namespace {
+// n_sink < 0: without sinks
+int prefill_entry(const lnskv_pages* c, const float* q, float* out, const int32_t* chunks, int32_t n_chunks,
+                  int32_t n_tok, const uint32_t* bt, int32_t bt_stride, int32_t n_rows, const int32_t* p_start,
+                  int32_t window, int32_t n_sink, int32_t n_heads, float scale, lnskv_stream_t stream) {
   clear_error();
   if (int rc = check_pages(c)) return rc;
   if (!q || !out || !chunks || !bt) return fail(LNSKV_ERR_INVALID, "q, out, chunks and block tables must be non-null");
@@ -1126,6 +1129,7 @@ int lnskv_prefill_attention(const lnskv_pages* c, const float* q, float* out, co
   a.bt = bt;
   a.p_start = p_start;
   a.window = window;
+  a.n_sink = n_sink;
   a.n_chunks = n_chunks;
   a.n_tok = n_tok;
   a.n_rows = n_rows;
@@ -1140,7 +1144,28 @@ int lnskv_prefill_attention(const lnskv_pages* c, const float* q, float* out, co
   const int64_t qt = prefill_queries_per_tile(rep, (int)c->head_dim);
   const int64_t tiles = ((int64_t)n_tok + qt - 1) / qt + n_chunks;
   if (tiles * c->n_kv_heads > INT32_MAX) return fail(LNSKV_ERR_INVALID, "too many query tiles");
+  if (n_sink >= 0) return launch_prefill_mfma_sink(a, rep, (int)c->head_dim, (int)tiles, (hipStream_t)stream);
   return launch_prefill_mfma(a, rep, (int)c->head_dim, (int)tiles, (hipStream_t)stream);
+}
+}  // namespace
+}  // namespace lnskv
+
+int lnskv_prefill_attention(const lnskv_pages* c, const float* q, float* out, const int32_t* chunks,
+                            int32_t n_chunks, int32_t n_tok, const uint32_t* bt, int32_t bt_stride, int32_t n_rows,
+                            const int32_t* p_start, int32_t window, int32_t n_heads, float scale,
+                            lnskv_stream_t stream) {
+  return prefill_entry(c, q, out, chunks, n_chunks, n_tok, bt, bt_stride, n_rows, p_start, window, -1, n_heads, scale,
+                       stream);
+}
+
+int lnskv_sink_prefill_attention(const lnskv_pages* c, const float* q, float* out, const int32_t* chunks,
+                                 int32_t n_chunks, int32_t n_tok, const uint32_t* bt, int32_t bt_stride,
+                                 int32_t n_rows, int32_t window, int32_t n_sink, int32_t n_heads, float scale,
+                                 lnskv_stream_t stream) {
+  clear_error();
+  if (n_sink < 0 || n_sink > (1 << 30)) return fail(LNSKV_ERR_INVALID, "n_sink %d out of range [0, 2^30]", n_sink);
+  return prefill_entry(c, q, out, chunks, n_chunks, n_tok, bt, bt_stride, n_rows, nullptr, window, n_sink, n_heads,
+                       scale, stream);
 }
 
 int lnskv_split_gated_query(const float* input, float* q_out, float* gate_out, int32_t n_rows, int32_t n_heads,

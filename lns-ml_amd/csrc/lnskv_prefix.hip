@@ -1,0 +1,425 @@
+// Decode attention of sequences that share a prefix: the shared pages are read
+// once for all query rows of a group, not once per sequence.
+//
+// softmax over [0, L) splits into the shared part [0, P) and the sequence's
+// own [P, L), each a numerator A = sum 2^(s - m) v, a sum l = sum 2^(s - m) and
+// a max m (s in log2 units); the two join as
+//   out = (2^(m1 - M) A1 + 2^(m2 - M) A2) / (2^(m1 - M) l1 + 2^(m2 - M) l2).
+// 1. prefix kernel: work item = (group, tile of the group's query rows, split of its
+//    pages, kv head).  A row is one query head of one sequence; all rows of a
+//    tile multiply the same K and V.  Each item leaves a partial row (A, m, l).
+// 2. merge kernel, when some group's pages are split: one partial row per query head.
+// 3. the decode kernels' kPrefix variant over [P, L): the piece that starts a
+//    sequence's segment merges its prefix row.
+#include "lnskv_decode_var.h"
+
+namespace lnskv {
+namespace {
+
+constexpr int kRowsTile = 64;   // query rows per tile: four waves of 16
+constexpr int kSplitPages = 4;  // fewest pages of a split
+
+struct PrefixArgs {
+  const uint8_t* k_pages;
+  const uint8_t* v_pages;
+  const float* k_scales;
+  const float* v_scales;
+  const float* q;         // [n_seq][n_heads][D]
+  const uint32_t* bt;     // [n_seq][bt_stride]
+  const int32_t* kv_len;  // [n_seq]
+  float* seed_acc;        // [n_seq][n_heads][D]: the groups' result
+  float* seed_ml;         // [n_seq][n_heads][2]
+  float* part_acc;        // partial rows of the groups with more than one split
+  float* part_ml;
+  int32_t bt_stride;
+  int32_t n_kv;
+  int32_t n_heads;
+  int32_t rep;
+  int32_t max_kv_len;
+  int32_t split_pages;  // pages per split
+  int32_t n_groups;
+  uint32_t num_pages;
+  float scale_log2;
+  PrefixGroup g[LNSKV_PREFIX_MAX_GROUPS];
+};
+
+__host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Item `i` of the launch (without its kv head): group, row tile and split, and
+// the partial rows of the groups before it.
+struct PrefixItem {
+  int group, tile, split, splits;
+  size_t part0;  // first partial row of the group
+};
+__device__ __forceinline__ PrefixItem prefix_item(const PrefixArgs& a, int i, int tile_rows) {
+  PrefixItem it{-1, 0, 0, 1, 0};
+  for (int g = 0; g < a.n_groups; ++g) {  // block-uniform
+    const int rows = (a.g[g].end - a.g[g].first) * a.rep;
+    const int tiles = ceil_div(rows, tile_rows), splits = ceil_div(a.g[g].pages, a.split_pages);
+    if (i < tiles * splits) {
+      it.group = g;
+      it.tile = i / splits;
+      it.split = i - it.tile * splits;
+      it.splits = splits;
+      return it;
+    }
+    i -= tiles * splits;
+    if (splits > 1) it.part0 += (size_t)rows * a.n_kv * splits;
+  }
+  return it;
+}
+
+// Where row (sequence s, query head h) of an item goes: its seed row, or its
+// partial row [row of the group][split].
+struct RowOut {
+  float* acc;
+  float* ml;
+};
+template <int D>
+__device__ __forceinline__ RowOut row_out(const PrefixArgs& a, const PrefixItem& it, int s, int h) {
+  const size_t hrow = (size_t)s * a.n_heads + h;
+  if (it.splits == 1) return {a.seed_acc + hrow * D, a.seed_ml + 2 * hrow};
+  const size_t r = it.part0 + ((size_t)(s - a.g[it.group].first) * a.n_heads + h) * it.splits + it.split;
+  return {a.part_acc + r * D, a.part_ml + 2 * r};
+}
+
+// Tokens of the prefix that sequence s attends: all of them unless its length
+// ends inside; none for a length out of range.
+__device__ __forceinline__ int row_tokens(const PrefixArgs& a, int s, int pages) {
+  const int L = a.kv_len[s];
+  return L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : min(max(L, 0), pages * kPage);
+}
+
+// ---------------------------------------------------------------------------
+// Every page type and head dim, in f32: both products as v_mfma_f32_16x16x4_f32
+// over a page of K and V held in LDS as f32 (Q8A: code x scale).  Wave w holds
+// rows 16w .. 16w + 15 of the tile.  Lane (g, n) = (lane / 16, lane % 16):
+//  S^T[16 tok][16 row] = K . Q^T, product (jj, e) over dims 16 jj + 4 g' + e
+//  (g' = 0..3 the contraction index), so that both operands of four products
+//  are one 16-byte read; lane (g, n) gets tokens 4g + ii of row n.
+//  O[16 row][D] += P . V, product ii over tokens 4 g' + ii: its A operand is the
+//  lane's own weight ii; lane (g, n) accumulates O[row 4g + i][16 nb + n].
+// LDS rows are D + 4 floats: four rows apart fall 16 banks apart.
+template <int DT, int D>
+__global__ __launch_bounds__(kBlock) void prefix_f32_kernel(PrefixArgs a) {
+  constexpr int ES = Storage<DT>::kBytes;
+  constexpr int kStride = D + 4;
+  constexpr int kElems = D / 16;              // elements of a row per thread
+  constexpr int kWords = kElems * ES / 4;     // and their 32-bit words (1 to 16)
+  __shared__ __attribute__((aligned(16))) float ks_[kPage * kStride];
+  __shared__ __attribute__((aligned(16))) float vs_[kPage * kStride];
+  __shared__ int most_[kWavesPerBlock];
+  const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
+  const PrefixItem it = prefix_item(a, (int)(blockIdx.x / (unsigned)a.n_kv), kRowsTile);
+  if (it.group < 0) return;  // block-uniform
+  const PrefixGroup gr = a.g[it.group];
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane >> 4, n = lane & 15;
+  const int rows = (gr.end - gr.first) * a.rep;
+  const int r0 = it.tile * kRowsTile + 16 * w;  // this wave's first row
+  const int pg0 = it.split * a.split_pages, pg_end = min(gr.pages, pg0 + a.split_pages);
+
+  const int rn = min(r0 + n, rows - 1);  // past the last row: that row again, never written
+  const int sn = gr.first + rn / a.rep, hn = kvh * a.rep + rn % a.rep;
+  const int limit = row_tokens(a, sn, gr.pages);
+  // tokens past every row's length are masked in the whole tile: their V is
+  // zeroed, since 0 * NaN of a stale slot would reach the sums
+  int most = limit;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o, kWave));
+  if (lane == 0) most_[w] = most;
+  __syncthreads();
+  most = max(max(most_[0], most_[1]), max(most_[2], most_[3]));
+  const int pg1 = min(pg_end, (most + kPage - 1) / kPage);
+  float4v q[D / 16];
+  {
+    const float4v* src = reinterpret_cast<const float4v*>(a.q + ((size_t)sn * a.n_heads + hn) * D) + g;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) q[j] = src[4 * j] * a.scale_log2;
+  }
+  float4v acc[D / 16];
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) acc[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kMInit, l = 0.0f;
+
+  // this thread's elements of a page: kElems of token threadIdx.x / 16
+  const int tt = threadIdx.x >> 4, tc = (threadIdx.x & 15) * kElems;
+  uint32_t kw[kWords], vw[kWords];
+  float ksc = 1.0f, vsc = 1.0f;
+  bool ok = false;
+  const uint32_t* bt_row = a.bt + (size_t)gr.first * a.bt_stride;
+  auto load = [&](int pg) {
+    const uint32_t ph = pg < a.bt_stride ? bt_row[pg] : 0xFFFFFFFFu;
+    ok = ph < a.num_pages;
+    const size_t slot = (size_t)(ok ? ph : 0u) * kPage + tt;  // a missing page reads page 0, masked
+    const size_t off = ((slot * a.n_kv + kvh) * D + tc) * ES;
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.k_pages + off);
+    const uint32_t* vp = reinterpret_cast<const uint32_t*>(a.v_pages + off);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      kw[i] = kp[i];
+      vw[i] = vp[i];
+    }
+    if constexpr (DT == LNSKV_DTYPE_Q8A) {
+      ksc = a.k_scales[slot * a.n_kv + kvh];
+      vsc = a.v_scales[slot * a.n_kv + kvh];
+    }
+  };
+  auto value = [](const uint32_t* word, int e, float sc) -> float {
+    const uint32_t x = word[e * ES / 4];
+    if constexpr (DT == LNSKV_DTYPE_F32) return __builtin_bit_cast(float, x);
+    else if constexpr (DT == LNSKV_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(x >> (16 * (e & 1))));
+    else return (float)(int8_t)(x >> (8 * (e & 3))) * sc;
+  };
+  if (pg0 < pg1) load(pg0);
+  for (int pg = pg0; pg < pg1; ++pg) {
+    const bool valid = ok;
+    __syncthreads();  // every wave is done with the page before
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) {
+      ks_[tt * kStride + tc + e] = value(kw, e, ksc);
+      vs_[tt * kStride + tc + e] = valid && pg * kPage + tt < most ? value(vw, e, vsc) : 0.0f;
+    }
+    __syncthreads();
+    if (pg + 1 < pg1) load(pg + 1);
+    float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      const float4v k = *reinterpret_cast<const float4v*>(ks_ + n * kStride + 16 * j + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[j][e], s, 0, 0, 0);
+    }
+    const int tok0 = pg * kPage;
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii)
+      if (!(valid && tok0 + 4 * g + ii < limit)) s[ii] = -INFINITY;
+    float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    mx = max_xor16(max_xor32(mx));  // over the page's tokens, row n
+    if (__builtin_amdgcn_ballot_w64(mx > m)) {  // wave-uniform
+      const float mn = fmaxf(m, mx), alpha = fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float ar = __shfl(alpha, 20 * g + i, kWave);  // row 4g + i
+#pragma unroll
+        for (int nb = 0; nb < D / 16; ++nb) acc[nb][i] *= ar;
+      }
+    }
+    float p[4];
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) p[ii] = fast_exp2(s[ii] - m);
+    l += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii)
+#pragma unroll
+      for (int nb = 0; nb < D / 16; ++nb)
+        acc[nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[ii], vs_[(4 * g + ii) * kStride + 16 * nb + n], acc[nb], 0, 0, 0);
+  }
+  l = sum_xor16(sum_xor32(l));
+  if (lane < 16 && r0 + n < rows) {
+    const RowOut o = row_out<D>(a, it, sn, hn);
+    o.ml[0] = m;
+    o.ml[1] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + 4 * g + i;
+    if (r < rows) {
+      const RowOut o = row_out<D>(a, it, gr.first + r / a.rep, kvh * a.rep + r % a.rep);
+#pragma unroll
+      for (int nb = 0; nb < D / 16; ++nb) o.acc[16 * nb + n] = acc[nb][i];
+    }
+  }
+}
+
+// One partial row per query head of a group whose pages are split: wave per
+// (sequence, head), the splits in order.
+template <int D>
+__global__ __launch_bounds__(kBlock) void prefix_merge_kernel(PrefixArgs a) {
+  constexpr int C = D / kWave;
+  int i = (int)blockIdx.x * kWavesPerBlock + (int)(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  size_t part0 = 0;
+  for (int g = 0; g < a.n_groups; ++g) {
+    const int rows = (a.g[g].end - a.g[g].first) * a.n_heads, splits = ceil_div(a.g[g].pages, a.split_pages);
+    if (splits <= 1) continue;
+    if (i < rows) {  // wave-uniform
+      const size_t base = part0 + (size_t)i * splits;
+      float M, Ls, A[C];
+      merge_wave<D, 1, 8>(reinterpret_cast<const float2*>(a.part_ml), a.part_acc, 0, splits,
+                          [=](int j) { return base + (size_t)j; }, M, Ls, A);
+      const size_t hrow = (size_t)a.g[g].first * a.n_heads + i;
+#pragma unroll
+      for (int c = 0; c < C; ++c) a.seed_acc[hrow * D + c * kWave + lane] = A[c];
+      if (lane == 0) {
+        a.seed_ml[2 * hrow] = M;
+        a.seed_ml[2 * hrow + 1] = Ls;
+      }
+      return;
+    }
+    i -= rows;
+    part0 += (size_t)rows * splits;
+  }
+}
+
+template <int DT>
+void launch_prefix_f32(const PrefixArgs& a, int d, unsigned blocks, hipStream_t st) {
+  switch (d) {
+    case 64: prefix_f32_kernel<DT, 64><<<blocks, kBlock, 0, st>>>(a); break;
+    case 128: prefix_f32_kernel<DT, 128><<<blocks, kBlock, 0, st>>>(a); break;
+    default: prefix_f32_kernel<DT, 256><<<blocks, kBlock, 0, st>>>(a); break;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The host's view of a call.
+struct PrefixPlan {
+  VarPlan own;            // the decode over the sequences' own pages
+  int64_t units = 0;      // and its units at most
+  int split_pages = 0;    // 0: nothing is shared
+  int64_t items = 0;      // work items per kv head
+  int64_t merge_rows = 0; // query heads of split groups
+  int64_t part_rows = 0;  // partial rows
+  size_t seed_at = 0, part_at = 0, ws_bytes = 0;
+  int n_groups = 0;
+  PrefixGroup g[LNSKV_PREFIX_MAX_GROUPS];
+};
+
+int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n_seq, int n_heads, int max_kv_len,
+                PrefixPlan* p) {
+  if (n_groups < 0 || n_groups > LNSKV_PREFIX_MAX_GROUPS)
+    return fail(LNSKV_ERR_INVALID, "n_groups %d out of range [0, %d]", n_groups, LNSKV_PREFIX_MAX_GROUPS);
+  if (n_groups > 0 && !groups) return fail(LNSKV_ERR_INVALID, "groups must be non-null");
+  const int rep = n_heads / (int)c->n_kv_heads, d = (int)c->head_dim;
+  const int64_t all = (int64_t)max_kv_len / kPage + 1;
+  int64_t own_pages = 0, most = 0, tiles = 0, max_shared = 0;  // summed over sequences; of one sequence
+  int at = 0;
+  for (int i = 0; i < n_groups; ++i) {
+    const int first = groups[3 * i], n = groups[3 * i + 1], tok = groups[3 * i + 2];
+    if (first < at || n <= 0 || n > n_seq - first || tok < 0)
+      return fail(LNSKV_ERR_INVALID,
+                  "group %d {%d, %d, %d}: groups lie in [0, %d), in order and apart, with tokens >= 0", i, first, n, tok,
+                  n_seq);
+    if (first > at) most = all;
+    own_pages += (first - at) * all;
+    at = first + n;
+    const int64_t shared = std::min<int64_t>(tok / kPage, all);
+    own_pages += n * std::max<int64_t>(all - shared, 1);
+    most = std::max(most, std::max<int64_t>(all - shared, 1));
+    if (shared == 0) continue;
+    p->g[p->n_groups++] = PrefixGroup{first, at, (int32_t)shared};
+    tiles += ceil_div(n * rep, kRowsTile);
+    max_shared = std::max(max_shared, shared);
+  }
+  if (at < n_seq) most = all;
+  own_pages += (n_seq - at) * all;
+  p->units = own_pages * c->n_kv_heads;
+  if (int rc = plan_var<kPrefix>(c, n_seq, n_heads, p->units, most, p->n_groups == 0, &p->own)) return rc;
+  p->ws_bytes = p->own.ws_bytes;
+  if (p->n_groups == 0) return LNSKV_OK;
+  // splits of equal pages, about two items per compute unit
+  const int64_t want = std::max<int64_t>(1, 512 / (tiles * c->n_kv_heads));
+  p->split_pages = (int)std::max<int64_t>(kSplitPages, (max_shared + want - 1) / want);
+  for (int i = 0; i < p->n_groups; ++i) {
+    const int64_t n = p->g[i].end - p->g[i].first, splits = ceil_div(p->g[i].pages, p->split_pages);
+    p->items += ceil_div((int)(n * rep), kRowsTile) * splits;
+    if (splits > 1) {
+      p->merge_rows += n * n_heads;
+      p->part_rows += n * n_heads * splits;
+    }
+  }
+  if (p->items * c->n_kv_heads > INT32_MAX) return fail(LNSKV_ERR_INVALID, "too many row tiles");
+  p->seed_at = (std::max(p->ws_bytes, kWsHeaderBytes) + 255) & ~(size_t)255;
+  p->part_at = p->seed_at + (((size_t)n_seq * n_heads * (d + 2) * sizeof(float) + 255) & ~(size_t)255);
+  p->ws_bytes = p->part_at + (size_t)p->part_rows * (d + 2) * sizeof(float);
+  return LNSKV_OK;
+}
+
+}  // namespace
+}  // namespace lnskv
+
+using namespace lnskv;
+
+extern "C" {
+
+int lnskv_prefix_decode_workspace_size(const lnskv_pages* c, const int32_t* groups, int32_t n_groups, int32_t n_seq,
+                                       int32_t n_heads, int32_t max_kv_len, size_t* bytes) {
+  clear_error();
+  if (!bytes) return fail(LNSKV_ERR_INVALID, "bytes is NULL");
+  *bytes = 0;
+  if (int rc = check_geometry(c)) return rc;
+  if (int rc = check_var_shape(c, n_seq, n_heads, max_kv_len)) return rc;
+  PrefixPlan p;
+  if (int rc = plan_prefix(c, groups, n_groups, n_seq, n_heads, max_kv_len, &p)) return rc;
+  *bytes = p.ws_bytes;
+  return LNSKV_OK;
+}
+
+int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const float* gate, const uint32_t* bt,
+                        int32_t bt_stride, const int32_t* kv_len, const int32_t* groups, int32_t n_groups,
+                        int32_t n_seq, int32_t n_heads, int32_t max_kv_len, float scale, void* ws, size_t ws_bytes,
+                        lnskv_stream_t stream) {
+  clear_error();
+  if (int rc = check_var_call(c, q, out, bt, bt_stride, kv_len, n_seq, n_heads, max_kv_len, scale)) return rc;
+  if (int rc = check_var_shape(c, n_seq, n_heads, max_kv_len)) return rc;
+  PrefixPlan p;
+  if (int rc = plan_prefix(c, groups, n_groups, n_seq, n_heads, max_kv_len, &p)) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (int rc = var_workspace(&ws, ws_bytes, p.ws_bytes, st)) return rc;
+  const DecodeArgs a = var_args(c, q, out, gate, bt, bt_stride, kv_len, n_heads, max_kv_len, scale, p.own, stream);
+  const int d = (int)c->head_dim;
+  float *seed_acc = nullptr, *seed_ml = nullptr;
+  if (p.n_groups > 0) {
+    uint8_t* base = static_cast<uint8_t*>(ws);
+    PrefixArgs x{};
+    x.k_pages = a.k_pages;
+    x.v_pages = a.v_pages;
+    x.k_scales = a.k_scales;
+    x.v_scales = a.v_scales;
+    x.q = q;
+    x.bt = bt;
+    x.kv_len = kv_len;
+    x.seed_acc = seed_acc = reinterpret_cast<float*>(base + p.seed_at);
+    x.seed_ml = seed_ml = seed_acc + (size_t)n_seq * n_heads * d;
+    x.part_acc = reinterpret_cast<float*>(base + p.part_at);
+    x.part_ml = x.part_acc + (size_t)p.part_rows * d;
+    x.bt_stride = bt_stride;
+    x.n_kv = a.n_kv;
+    x.n_heads = n_heads;
+    x.rep = n_heads / a.n_kv;
+    x.max_kv_len = max_kv_len;
+    x.split_pages = p.split_pages;
+    x.n_groups = p.n_groups;
+    x.num_pages = c->num_pages;
+    x.scale_log2 = a.scale_log2;
+    std::copy(p.g, p.g + p.n_groups, x.g);
+    const unsigned blocks = (unsigned)(p.items * a.n_kv);
+    switch (c->dtype) {
+      case LNSKV_DTYPE_F32: launch_prefix_f32<LNSKV_DTYPE_F32>(x, d, blocks, st); break;
+      case LNSKV_DTYPE_F16: launch_prefix_f32<LNSKV_DTYPE_F16>(x, d, blocks, st); break;
+      default: launch_prefix_f32<LNSKV_DTYPE_Q8A>(x, d, blocks, st); break;
+    }
+    if (int rc = hip_check("prefix kernel launch")) return rc;
+    if (p.merge_rows > 0) {
+      const unsigned mb = (unsigned)((p.merge_rows + kWavesPerBlock - 1) / kWavesPerBlock);
+      switch (d) {
+        case 64: prefix_merge_kernel<64><<<mb, kBlock, 0, st>>>(x); break;
+        case 128: prefix_merge_kernel<128><<<mb, kBlock, 0, st>>>(x); break;
+        default: prefix_merge_kernel<256><<<mb, kBlock, 0, st>>>(x); break;
+      }
+      if (int rc = hip_check("prefix merge kernel launch")) return rc;
+    }
+  }
+  return launch_plan<kPrefix>(c, a, p.own, p.units, n_seq, ws, st, [&](int s0) {
+    VarArgs<kPrefix> x{};
+    const size_t r = (size_t)s0 * n_heads;
+    x.seed_acc = seed_acc ? seed_acc + r * d : nullptr;
+    x.seed_ml = seed_ml ? seed_ml + 2 * r : nullptr;
+    x.s0 = s0;
+    x.n_groups = p.n_groups;
+    std::copy(p.g, p.g + p.n_groups, x.g);
+    return x;
+  });
+}
+
+}  // extern "C"

@@ -23,6 +23,8 @@ pub const LNSKV_Q4L_DISK_BYTES: usize = 134;
 pub const LNSKV_Q4L_DEVICE_BYTES: usize = 144;
 /// `LNSKV_TABLE_PATCH_MAX`: changed block-table entries one patch writes by value.
 pub const LNSKV_TABLE_PATCH_MAX: usize = 64;
+/// `LNSKV_PREFIX_MAX_GROUPS`: groups of sequences one `lnskv_prefix_decode` takes.
+pub const LNSKV_PREFIX_MAX_GROUPS: usize = 128;
 
 /// `lnskv_dtype`.
 pub const LNSKV_DTYPE_F32: i32 = 0;
@@ -236,6 +238,96 @@ extern "C" {
         scale: f32,
         stream: HipStream,
     ) -> c_int;
+    pub fn lnskv_mrope_append(
+        c: *const LnskvPages,
+        rope: *const LnskvRope,
+        sections: *const i32,
+        n_axes: i32,
+        interleaved: i32,
+        q_dev: *const f32,
+        q_out_dev: *mut f32,
+        n_heads: i32,
+        k_new_dev: *const f32,
+        v_new_dev: *const f32,
+        axis_pos_dev: *const i32,
+        tok_seq_dev: *const i32,
+        tok_pos_dev: *const i32,
+        n_tok: i32,
+        block_tables_dev: *const u32,
+        bt_stride: i32,
+        n_rows: i32,
+        stream: HipStream,
+    ) -> c_int;
+    pub fn lnskv_sink_decode_workspace_size(
+        c: *const LnskvPages,
+        n_seq: i32,
+        n_heads: i32,
+        max_kv_len: i32,
+        window: i32,
+        n_sink: i32,
+        bytes: *mut usize,
+    ) -> c_int;
+    pub fn lnskv_sink_decode(
+        c: *const LnskvPages,
+        q_dev: *const f32,
+        out_dev: *mut f32,
+        gate_dev: *const f32,
+        block_tables_dev: *const u32,
+        bt_stride: i32,
+        kv_len_dev: *const i32,
+        n_seq: i32,
+        n_heads: i32,
+        max_kv_len: i32,
+        window: i32,
+        n_sink: i32,
+        scale: f32,
+        workspace_dev: *mut c_void,
+        ws_bytes: usize,
+        stream: HipStream,
+    ) -> c_int;
+    pub fn lnskv_sink_prefill_attention(
+        c: *const LnskvPages,
+        q_dev: *const f32,
+        out_dev: *mut f32,
+        chunks_dev: *const i32,
+        n_chunks: i32,
+        n_tok: i32,
+        block_tables_dev: *const u32,
+        bt_stride: i32,
+        n_rows: i32,
+        window: i32,
+        n_sink: i32,
+        n_heads: i32,
+        scale: f32,
+        stream: HipStream,
+    ) -> c_int;
+    pub fn lnskv_prefix_decode_workspace_size(
+        c: *const LnskvPages,
+        groups: *const i32,
+        n_groups: i32,
+        n_seq: i32,
+        n_heads: i32,
+        max_kv_len: i32,
+        bytes: *mut usize,
+    ) -> c_int;
+    pub fn lnskv_prefix_decode(
+        c: *const LnskvPages,
+        q_dev: *const f32,
+        out_dev: *mut f32,
+        gate_dev: *const f32,
+        block_tables_dev: *const u32,
+        bt_stride: i32,
+        kv_len_dev: *const i32,
+        groups: *const i32,
+        n_groups: i32,
+        n_seq: i32,
+        n_heads: i32,
+        max_kv_len: i32,
+        scale: f32,
+        workspace_dev: *mut c_void,
+        ws_bytes: usize,
+        stream: HipStream,
+    ) -> c_int;
     pub fn lnskv_split_gated_query(
         input_dev: *const f32,
         q_out_dev: *mut f32,
@@ -375,6 +467,34 @@ extern "C" {
         window: i32,
     ) -> c_int;
     pub fn lnskv_window_pages(window: i32) -> i32;
+    pub fn lnskv_evict_kv_pages_sink(
+        t: *mut LnskvBlockTables,
+        pool: *mut LnskvPagePool,
+        seq: i32,
+        pos: i32,
+        window: i32,
+        n_sink: i32,
+    ) -> c_int;
+    pub fn lnskv_step_pages_sink(
+        t: *mut LnskvBlockTables,
+        pool: *mut LnskvPagePool,
+        layer: i32,
+        seq: i32,
+        pos: i32,
+        window: i32,
+        n_sink: i32,
+    ) -> c_int;
+    pub fn lnskv_sink_window_pages(
+        window: i32,
+        n_sink: i32,
+    ) -> i32;
+    pub fn lnskv_shared_prefix_groups(
+        t: *const LnskvBlockTables,
+        n_seq: i32,
+        min_pages: i32,
+        groups: *mut i32,
+        n_groups: *mut i32,
+    ) -> c_int;
     pub fn lnskv_free_sequence(t: *mut LnskvBlockTables, pool: *mut LnskvPagePool, seq: i32) -> c_int;
     pub fn lnskv_fork_sequence(
         t: *mut LnskvBlockTables,

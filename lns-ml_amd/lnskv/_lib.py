@@ -33,6 +33,9 @@ TABLE_PATCH_MAX = 64
 # (the workgroup schedule's counters; every call leaves them zero)
 WORKSPACE_HEADER_BYTES = 4096
 
+# groups of sequences that one lnskv_prefix_decode takes
+PREFIX_MAX_GROUPS = 128
+
 
 class LnskvError(RuntimeError):
     """A non-zero lnskv_status with the library's message (the reference's
@@ -128,6 +131,20 @@ SIGNATURES = {
         C.c_int, [_P, _R, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _i32, _vp, _sz, _vp]),
     "lnskv_prefill_attention": (C.c_int, [_P, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _f32,
                                           _vp]),
+    "lnskv_mrope_append": (
+        C.c_int, [_P, _R, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp]),
+    "lnskv_sink_decode_workspace_size": (C.c_int, [_P, _i32, _i32, _i32, _i32, _i32, C.POINTER(_sz)]),
+    "lnskv_sink_decode": (
+        C.c_int, [_P, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
+    "lnskv_sink_prefill_attention": (
+        C.c_int, [_P, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "lnskv_prefix_decode_workspace_size": (C.c_int, [_P, _vp, _i32, _i32, _i32, _i32, C.POINTER(_sz)]),
+    "lnskv_prefix_decode": (
+        C.c_int, [_P, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
+    "lnskv_evict_kv_pages_sink": (C.c_int, [_vp, _vp, _i32, _i32, _i32, _i32]),
+    "lnskv_step_pages_sink": (C.c_int, [_vp, _vp, _i32, _i32, _i32, _i32, _i32]),
+    "lnskv_sink_window_pages": (_i32, [_i32, _i32]),
+    "lnskv_shared_prefix_groups": (C.c_int, [_vp, _i32, _i32, _vp, C.POINTER(_i32)]),
     "lnskv_split_gated_query": (C.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     "lnskv_gated_append_decode": (
         C.c_int, [_P, _R, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _i32, _vp, _sz,

@@ -24,6 +24,28 @@ def _stream(device: torch.device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class _on:
+    """Makes a device current for a call (streams and workspaces are per device);
+    nothing when it is already."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = None
+        if self.index is not None:
+            now = torch.cuda.current_device()
+            if now != self.index:
+                self.before = now
+                torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+
+
 def _need(t: torch.Tensor, name: str, dtype, numel: int, device) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
@@ -76,6 +98,7 @@ class PagedKV:
                           self.ks.data_ptr() if self.ks is not None else None,
                           self.vs.data_ptr() if self.vs is not None else None,
                           num_pages, n_kv_heads, head_dim, dtype)
+        self._c = C.byref(self.desc)
 
     # -- helpers -------------------------------------------------------------
     @property
@@ -88,6 +111,26 @@ class PagedKV:
         _need(tables, "block_tables", torch.int32 if tables.dtype == torch.int32 else torch.uint32,
               tables.numel(), self.device)
         return int(tables.shape[1])
+
+    def _any_tables(self, tables: torch.Tensor) -> int:
+        """Block tables of any number of rows; returns their stride."""
+        if tables.dim() != 2 or tables.dtype not in (torch.int32, torch.uint32):
+            raise ValueError("block tables must be 2-D, int32 or uint32")
+        _need(tables, "block_tables", tables.dtype, tables.numel(), self.device)
+        return int(tables.shape[1])
+
+    def _variant_common(self, q, tables, kv_len, n_heads, gate, workspace, out):
+        n_seq, stride = self._decode_common(q, tables, kv_len, None, n_heads)
+        if gate is not None:
+            _need(gate, "gate", torch.float32, q.numel(), self.device)
+        if out is None:
+            out = torch.empty((n_seq, n_heads, self.head_dim), dtype=torch.float32, device=self.device)
+        _need(out, "out", torch.float32, q.numel(), self.device)
+        if workspace is None:
+            return n_seq, stride, out, 0
+        ws_bytes = workspace.numel() * workspace.element_size()
+        _need(workspace, "workspace", workspace.dtype, workspace.numel(), self.device)
+        return n_seq, stride, out, ws_bytes
 
     # -- operations ----------------------------------------------------------
     def clear(self) -> None:
@@ -237,6 +280,95 @@ class PagedKV:
                                             _stream(self.device)))
         return out
 
+    def mrope_append(self, rope: "MRopeTable", k_new, v_new, axis_pos, tok_seq, tok_pos, tables, q=None,
+                     q_out=None) -> torch.Tensor | None:
+        """lnskv_mrope_append: K (turned by the positions axis_pos [n_axes][n_tok])
+        and V of every token into the slots of tok_pos; q [n_tok][n_heads][d], when
+        given, turned the same way into q_out (q itself, or None: a new tensor),
+        which is returned."""
+        n_tok = int(tok_seq.numel())
+        dev = self.device
+        _need(k_new, "k_new", torch.float32, n_tok * self.row_elems, dev)
+        _need(v_new, "v_new", torch.float32, n_tok * self.row_elems, dev)
+        _need(axis_pos, "axis_pos", torch.int32, rope.n_axes * n_tok, dev)
+        _need(tok_seq, "tok_seq", torch.int32, n_tok, dev)
+        _need(tok_pos, "tok_pos", torch.int32, n_tok, dev)
+        if rope.inv_freqs.device != dev:
+            raise ValueError(f"rope must be on {dev}, got {rope.inv_freqs.device}")
+        stride = self._any_tables(tables)
+        n_heads = 0
+        if q is not None:
+            if n_tok and q.numel() % (n_tok * self.head_dim):
+                raise ValueError("q must be [n_tok][n_heads][head_dim]")
+            n_heads = q.numel() // (n_tok * self.head_dim) if n_tok else self.n_kv
+            _need(q, "q", torch.float32, q.numel(), dev)
+            if q_out is None:
+                q_out = torch.empty_like(q)
+            _need(q_out, "q_out", torch.float32, q.numel(), dev)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        with _on(dev):
+            check(lib().lnskv_mrope_append(self._c, rope._c, rope._sections, rope.n_axes, rope.interleaved, _ptr(q),
+                                           _ptr(q_out), n_heads, _ptr(k_new), _ptr(v_new), _ptr(axis_pos),
+                                           _ptr(tok_seq), _ptr(tok_pos), n_tok, _ptr(tables), stride,
+                                           int(tables.shape[0]), _stream(dev)))
+        return q_out
+
+    def sink_workspace_size(self, n_seq: int, n_heads: int, max_kv_len: int, window: int, n_sink: int) -> int:
+        out = C.c_size_t()
+        with _on(self.device):
+            check(lib().lnskv_sink_decode_workspace_size(self._c, n_seq, n_heads, max_kv_len, window, n_sink,
+                                                         C.byref(out)))
+        return out.value
+
+    def sink_decode(self, q, tables, kv_len, *, n_heads: int, max_kv_len: int, scale: float, window: int,
+                    n_sink: int, gate=None, workspace=None, out=None) -> torch.Tensor:
+        """lnskv_sink_decode: every sequence attends its first n_sink tokens and its
+        last `window` (0: all of them)."""
+        n_seq, stride, out, ws_bytes = self._variant_common(q, tables, kv_len, n_heads, gate, workspace, out)
+        with _on(self.device):
+            check(lib().lnskv_sink_decode(self._c, _ptr(q), _ptr(out), _ptr(gate), _ptr(tables), stride, _ptr(kv_len),
+                                          n_seq, n_heads, max_kv_len, window, n_sink, scale, _ptr(workspace),
+                                          ws_bytes, _stream(self.device)))
+        return out
+
+    def sink_prefill_attention(self, q, chunks, tables, *, n_heads: int, scale: float, window: int, n_sink: int,
+                               out=None) -> torch.Tensor:
+        """lnskv_sink_prefill_attention: prefill_attention whose queries attend the
+        first n_sink tokens besides their own window."""
+        n_tok = q.numel() // (n_heads * self.head_dim)
+        _need(q, "q", torch.float32, n_tok * n_heads * self.head_dim, self.device)
+        if chunks.dim() != 2 or chunks.shape[1] != 4:
+            raise ValueError("chunks must be [n_chunks][4]")
+        _need(chunks, "chunks", torch.int32, chunks.numel(), self.device)
+        stride = self._any_tables(tables)
+        if out is None:
+            out = torch.empty((n_tok, n_heads, self.head_dim), dtype=torch.float32, device=self.device)
+        _need(out, "out", torch.float32, q.numel(), self.device)
+        with _on(self.device):
+            check(lib().lnskv_sink_prefill_attention(self._c, _ptr(q), _ptr(out), _ptr(chunks), int(chunks.shape[0]),
+                                                     n_tok, _ptr(tables), stride, int(tables.shape[0]), window,
+                                                     n_sink, n_heads, scale, _stream(self.device)))
+        return out
+
+    def prefix_workspace_size(self, groups: "PrefixGroups", n_seq: int, n_heads: int, max_kv_len: int) -> int:
+        out = C.c_size_t()
+        with _on(self.device):
+            check(lib().lnskv_prefix_decode_workspace_size(self._c, groups._p, groups.n, n_seq, n_heads, max_kv_len,
+                                                           C.byref(out)))
+        return out.value
+
+    def prefix_decode(self, q, tables, kv_len, groups: "PrefixGroups", *, n_heads: int, max_kv_len: int,
+                      scale: float, gate=None, workspace=None, out=None) -> torch.Tensor:
+        """lnskv_prefix_decode: decode in which the sequences of each group read
+        their shared leading pages once for all (from the group's first row)."""
+        n_seq, stride, out, ws_bytes = self._variant_common(q, tables, kv_len, n_heads, gate, workspace, out)
+        with _on(self.device):
+            check(lib().lnskv_prefix_decode(self._c, _ptr(q), _ptr(out), _ptr(gate), _ptr(tables), stride,
+                                            _ptr(kv_len), groups._p, groups.n, n_seq, n_heads, max_kv_len, scale,
+                                            _ptr(workspace), ws_bytes, _stream(self.device)))
+        return out
+
     def attention_paged(self, q, k_in, v_in, block_table, pos: int, n_heads: int, p_start: int = 0,
                         out=None, dispatch: bool = False) -> torch.Tensor:
         """The reference's single-sequence call (encode_attention_paged_q8a,
@@ -297,6 +429,34 @@ class RopeTable:
         self.desc = Rope(self.inv_freqs.data_ptr(), rotary_dim)
 
 
+class MRopeTable:
+    """Rotary positions of several axes (lnskv_mrope_append): the inverse frequencies
+    (a float32 device tensor of rotary_dim / 2, e.g. RopeTable.inv_freqs), and how many
+    of those pairs each axis turns, in runs or (interleaved) dealt in turn."""
+
+    def __init__(self, inv_freqs: torch.Tensor, sections, interleaved: bool = False):
+        _need(inv_freqs, "inv_freqs", torch.float32, inv_freqs.numel(), inv_freqs.device)
+        self.inv_freqs = inv_freqs
+        self.rotary_dim = 2 * inv_freqs.numel()
+        self.sections = [int(x) for x in sections]
+        self.n_axes, self.interleaved = len(self.sections), int(bool(interleaved))
+        self.desc = Rope(inv_freqs.data_ptr(), self.rotary_dim)
+        self._c = C.byref(self.desc)
+        self._sections = (C.c_int32 * max(1, self.n_axes))(*self.sections)
+
+
+class PrefixGroups:
+    """Runs of sequences that share leading pages, as (first sequence, sequences, shared
+    tokens): what BlockTables.shared_prefix_groups returns."""
+
+    def __init__(self, groups):
+        rows = [tuple(int(x) for x in g) for g in groups]
+        if any(len(g) != 3 for g in rows):
+            raise ValueError("a group is (first sequence, sequences, shared tokens)")
+        self.groups, self.n = rows, len(rows)
+        self._p = (C.c_int32 * max(1, 3 * self.n))(*[x for g in rows for x in g])
+
+
 class Q4LMatrix:
     """A rows x cols Q4_L weight matrix on the device: the disk super-blocks
     (134 bytes per 256 weights, row-major) repacked by lnskv_q4l_prepare
@@ -341,4 +501,4 @@ def sync(device=None) -> None:
     check(lib().lnskv_sync(_stream(dev)))
 
 
-__all__ = ["PagedKV", "sync", "DTYPE_F32", "DTYPE_F16", "DTYPE_Q8A", "TORCH_DTYPE"]
+__all__ = ["PagedKV", "MRopeTable", "PrefixGroups", "sync", "DTYPE_F32", "DTYPE_F16", "DTYPE_Q8A", "TORCH_DTYPE"]

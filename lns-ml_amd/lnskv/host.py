@@ -11,7 +11,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import NO_PAGE, PAGE_SIZE, LnskvError, check, lib
+from ._lib import NO_PAGE, PAGE_SIZE, PREFIX_MAX_GROUPS, LnskvError, check, lib
 
 
 class PagePool:
@@ -115,6 +115,24 @@ class BlockTables:
         needs only window_pages(window) pages per sequence."""
         check(lib().lnskv_step_pages(self._h, pool.handle, layer, seq, pos, window))
 
+    def evict_kv_pages_sink(self, pool: PagePool, seq: int, pos: int, window: int, n_sink: int) -> None:
+        """evict_kv_pages that keeps the pages of the first n_sink tokens."""
+        check(lib().lnskv_evict_kv_pages_sink(self._h, pool.handle, seq, pos, window, n_sink))
+
+    def step_pages_sink(self, pool: PagePool, seq: int, pos: int, window: int, n_sink: int, layer: int = 0) -> None:
+        """lnskv_step_pages_sink: evict_kv_pages_sink then ensure_kv_page
+        (sink_window_pages(window, n_sink) pages per sequence)."""
+        check(lib().lnskv_step_pages_sink(self._h, pool.handle, layer, seq, pos, window, n_sink))
+
+    def shared_prefix_groups(self, n_seq: int | None = None, min_pages: int = 1) -> list[tuple[int, int, int]]:
+        """(first sequence, sequences, shared tokens) of the runs of rows that share
+        at least min_pages leading pages, for PagedKV.prefix_decode."""
+        out = np.zeros((PREFIX_MAX_GROUPS, 3), np.int32)
+        n = C.c_int32()
+        check(lib().lnskv_shared_prefix_groups(self._h, self.n_seq if n_seq is None else n_seq, min_pages,
+                                               out.ctypes.data_as(C.c_void_p), C.byref(n)))
+        return [tuple(int(x) for x in row) for row in out[:n.value]]
+
     def free_sequence(self, pool: PagePool, seq: int) -> None:
         check(lib().lnskv_free_sequence(self._h, pool.handle, seq))
 
@@ -147,4 +165,9 @@ def window_pages(window: int) -> int:
     return lib().lnskv_window_pages(window)
 
 
-__all__ = ["PagePool", "BlockTables", "kv_p_start", "window_pages", "LnskvError", "NO_PAGE", "PAGE_SIZE"]
+def sink_window_pages(window: int, n_sink: int) -> int:
+    """Pages per sequence that lnskv_step_pages_sink needs (0 for full attention)."""
+    return lib().lnskv_sink_window_pages(window, n_sink)
+
+
+__all__ = ["PagePool", "BlockTables", "kv_p_start", "window_pages", "sink_window_pages", "LnskvError", "NO_PAGE", "PAGE_SIZE"]
