@@ -5,21 +5,23 @@
 // own [P, L), each a numerator A = sum 2^(s - m) v, a sum l = sum 2^(s - m) and
 // a max m (s in log2 units); the two join as
 //   out = (2^(m1 - M) A1 + 2^(m2 - M) A2) / (2^(m1 - M) l1 + 2^(m2 - M) l2).
-// 1. prefix kernel: work item = (group, tile of the group's query rows, split of its
+// 1. prefix kernels: work item = (group, tile of the group's query rows, split of its
 //    pages, kv head).  A row is one query head of one sequence; all rows of a
 //    tile multiply the same K and V.  Each item leaves a partial row (A, m, l).
 // 2. merge kernel, when some group's pages are split: one partial row per query head.
 // 3. the decode kernels' kPrefix variant over [P, L): the piece that starts a
 //    sequence's segment merges its prefix row.
 #include "lnskv_decode_var.h"
+#include "lnskv_prefill.h"
 
 namespace lnskv {
 namespace {
 
-constexpr int kRowsTile = 64;   // query rows per tile: four waves of 16
+constexpr int kRowsTile = 64;   // query rows per tile of the f32 kernel: four waves of 16
 constexpr int kSplitPages = 4;  // fewest pages of a split
 
 struct PrefixArgs {
+  PrefillArgs pf;  // the pools, for the prefill kernel's page pipeline
   const uint8_t* k_pages;
   const uint8_t* v_pages;
   const float* k_scales;
@@ -56,10 +58,10 @@ __device__ __forceinline__ PrefixItem prefix_item(const PrefixArgs& a, int i, in
   for (int g = 0; g < a.n_groups; ++g) {  // block-uniform
     const int rows = (a.g[g].end - a.g[g].first) * a.rep;
     const int tiles = ceil_div(rows, tile_rows), splits = ceil_div(a.g[g].pages, a.split_pages);
-    if (i < tiles * splits) {
+    if (i < tiles * splits) {  // the tiles of one split side by side: they read the same pages
       it.group = g;
-      it.tile = i / splits;
-      it.split = i - it.tile * splits;
+      it.split = i / tiles;
+      it.tile = i - it.split * tiles;
       it.splits = splits;
       return it;
     }
@@ -91,7 +93,7 @@ __device__ __forceinline__ int row_tokens(const PrefixArgs& a, int s, int pages)
 }
 
 // ---------------------------------------------------------------------------
-// Every page type and head dim, in f32: both products as v_mfma_f32_16x16x4_f32
+// f32 pages, and 64-wide heads on every page type, in f32: both products as v_mfma_f32_16x16x4_f32
 // over a page of K and V held in LDS as f32 (Q8A: code x scale).  Wave w holds
 // rows 16w .. 16w + 15 of the tile.  Lane (g, n) = (lane / 16, lane % 16):
 //  S^T[16 tok][16 row] = K . Q^T, product (jj, e) over dims 16 jj + 4 g' + e
@@ -232,6 +234,207 @@ __global__ __launch_bounds__(kBlock) void prefix_f32_kernel(PrefixArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// f16 and Q8A pages with 128- or 256-wide heads, on the matrix cores: the
+// prefill kernel's page pipeline (eight waves, pairs of pages by DMA through an
+// LDS ring, q and the weights as pairs of f16) with query rows gathered from the
+// group's sequences.  Every row attends every token of the split, but for rows
+// whose length ends inside it.  Column n of wave w holds HW query heads of one
+// sequence (column u of the group: sequence u / (rep / HW), heads HW (u % (rep /
+// HW)) ..), so that its HW rows have the same length.  HW = 2 shares each K and V
+// operand read from LDS between two rows' tiles (NH = 1; a 256-wide head's
+// accumulators leave room for one).
+template <bool Q8, int NH, int HW>
+__global__ __launch_bounds__(kWave * 8) void prefix_mfma_kernel(PrefixArgs a) {
+  constexpr int D = NH * kD, NW = 8;
+  constexpr int kBatch = NH == 2 ? 1 : 2, kDepth = 3 * kBatch;
+  constexpr int RPW = Q8 ? NH + 2 : 16 * NH / NW;  // vector-memory instructions per wave and pair
+  constexpr int kRingSlot = Q8 ? kPfQ8Slot<NH> : kPfSlot<NH>;
+  __shared__ __attribute__((aligned(16))) uint8_t ring_[kDepth * kRingSlot];
+  __shared__ __attribute__((aligned(16))) uint8_t f16buf_[Q8 ? 2 * kBatch * kPfSlot<NH> : 16];
+  __shared__ int most_[NW];
+  const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
+  const PrefixItem it = prefix_item(a, (int)(blockIdx.x / (unsigned)a.n_kv), 16 * NW * HW);
+  if (it.group < 0) return;  // block-uniform
+  const PrefixGroup gr = a.g[it.group];
+  const int lane = (int)(threadIdx.x & (kWave - 1)), w = (int)(threadIdx.x / kWave);
+  const int g = lane >> 4, n = lane & 15;
+  const int per = a.rep / HW;                        // columns of a sequence
+  const int cols = (gr.end - gr.first) * per;
+  const int u0 = (it.tile * NW + w) * 16;            // this wave's first column
+  const bool active = u0 < cols;
+  // past the last column: that column again, never written
+  const int un = min(u0 + n, cols - 1);
+  const int sn = gr.first + un / per, hn = kvh * a.rep + un % per * HW;
+  const int limit = row_tokens(a, sn, gr.pages);  // tokens that column n attends
+  int most = limit, least = limit;
+
+  float4v qraw[HW][8 * NH];
+#pragma unroll
+  for (int hh = 0; hh < HW; ++hh) {
+    const float4v* src = reinterpret_cast<const float4v*>(a.q + ((size_t)sn * a.n_heads + hn + hh) * D + 8 * g);
+#pragma unroll
+    for (int j = 0; j < 4 * NH; ++j) {
+      qraw[hh][2 * j] = src[8 * j];
+      qraw[hh][2 * j + 1] = src[8 * j + 1];
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    most = max(most, __shfl_xor(most, o, kWave));
+    least = min(least, __shfl_xor(least, o, kWave));
+  }
+  if (lane == 0) most_[w] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NW; ++i) most = max(most, most_[i]);
+  const int pg_first = it.split * a.split_pages;
+  const int ta = pg_first * kPage, tb = min(min(gr.pages, pg_first + a.split_pages) * kPage, most);
+  const int npg = ta < tb ? (tb - 1) / kPage - pg_first + 1 : 0;
+  const int npairs = (npg + 1) / 2;
+
+  const uint32_t* bt_row = a.bt + (size_t)gr.first * a.bt_stride;
+  int base = pg_first;
+  uint32_t btv = 0;
+  auto load_window = [&]() {
+    const int e = base + lane;
+    btv = e < a.bt_stride ? bt_row[e] : 0xFFFFFFFFu;
+    wait_vmcnt<0>();
+  };
+  load_window();
+  auto phys_of = [&](int i) -> uint32_t {  // i increases from call to call
+    int idx = pg_first + i - base;
+    if (idx >= 64) {
+      base += 64;
+      idx -= 64;
+      load_window();
+    }
+    return __builtin_amdgcn_readlane(btv, idx);
+  };
+
+  PfLanes pl;
+  const uint32_t rs = (uint32_t)a.n_kv * (NH * kRowBytes);
+  const uint32_t page_bytes = kPage * rs;
+  const uint32_t kvh_off = (uint32_t)kvh * (NH * kRowBytes);
+  {
+    const int j = w & 3;  // this wave's quarter of a page region
+    const uint32_t R = 4u * (uint32_t)j + (uint32_t)g;
+    pl.koff = R * rs + 16u * ((uint32_t)n ^ R);
+    pl.voff = (uint32_t)(4 * g + j) * rs + 16u * ((uint32_t)n ^ v_swz((int)R));
+    pl.lds_q = 1024u * (uint32_t)j;
+    pl.krow = (uint32_t)n * kRowBytes + 16u * ((uint32_t)g ^ ((uint32_t)n & 3u));
+    pl.kx = 64u * ((uint32_t)n >> 2);
+    const int Rv = 4 * (n >> 2) + g;
+    pl.vrow = (uint32_t)Rv * kRowBytes + 8u * (n & 1) + 16u * (uint32_t)((n & 3) >> 1);
+    pl.vx = 16u * v_swz(Rv);
+  }
+  lds_u8* ring = (lds_u8*)ring_;
+  uint32_t vbits = 0;  // validity of the ring slots' pages
+  auto issue = [&](int i) {
+    const int sl = i % kDepth;
+    const uint32_t ph0 = phys_of(2 * i);
+    const uint32_t ph1 = 2 * i + 1 < npg ? phys_of(2 * i + 1) : 0xFFFFFFFFu;
+    const uint32_t bits = (ph0 < a.num_pages ? 1u : 0u) | (ph1 < a.num_pages ? 2u : 0u);
+    vbits = (vbits & ~(3u << (2 * sl))) | (bits << (2 * sl));
+    if constexpr (Q8)
+      pf_issue_q8<NH, true>(a.pf, (uint32_t)a.n_kv * D, (uint32_t)kvh, ring + sl * kRingSlot, ph0, ph1, w);
+    else
+      pf_issue<RPW>(a.pf, pl, page_bytes, kvh_off, ring + sl * kRingSlot, ph0, ph1, w);
+  };
+#pragma unroll
+  for (int i = 0; i < 2 * kBatch; ++i)
+    if (i < npairs) issue(i);
+
+  half8 qh[HW][4 * NH], ql[HW][4 * NH];
+  float qexp[HW], m[HW], l[HW];
+  float4v acc[HW][8 * NH];
+  float vnorm = 0.0f;  // Q8: acc is in units of vnorm
+#pragma unroll
+  for (int hh = 0; hh < HW; ++hh) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8 * NH; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(qraw[hh][r][e] * a.scale_log2));
+    amax = max_xor16(max_xor32(amax));
+    int E = 0;
+    if (amax > 0.0f && amax < INFINITY) (void)frexpf(amax, &E);
+    const float inv = ldexpf(1.0f, -E);
+    qexp[hh] = ldexpf(1.0f, E);
+#pragma unroll
+    for (int j = 0; j < 4 * NH; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = qraw[hh][2 * j + (e >> 2)][e & 3] * a.scale_log2 * inv;
+        const _Float16 hi = (_Float16)y;
+        qh[hh][j][e] = hi;
+        ql[hh][j][e] = (_Float16)(y - (float)hi);
+      }
+    m[hh] = kMInit;
+    l[hh] = 0.0f;
+#pragma unroll
+    for (int nb = 0; nb < 8 * NH; ++nb) acc[hh][nb] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  for (int i0 = 0; i0 < npairs; i0 += kBatch) {
+    const int later = min(max(npairs - (i0 + kBatch), 0), kBatch);  // pairs that may stay in flight
+    if (later == 2)
+      wait_vmcnt<2 * RPW>();
+    else if (later == 1)
+      wait_vmcnt<RPW>();
+    else
+      wait_vmcnt<0>();
+    lds_u8* f16b = (lds_u8*)f16buf_ + ((i0 / kBatch) & 1) * (kBatch * kPfSlot<NH>);
+    if constexpr (Q8) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (i0 + k < npairs) pf_convert_q8<NH>(ring + ((i0 + k) % kDepth) * kRingSlot, f16b + k * kPfSlot<NH>, w);
+    }
+    pf_barrier();  // every wave's quarters of this batch landed; the previous batch is consumed
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (i0 + 2 * kBatch + k < npairs) issue(i0 + 2 * kBatch + k);
+    for (int i = i0; i < min(i0 + kBatch, npairs); ++i) {
+      if (active) {
+        const int sl = i % kDepth;
+        lds_u8* sp = Q8 ? f16b + (i - i0) * kPfSlot<NH> : ring + sl * kRingSlot;
+        const lds_u8* sc = ring + sl * kRingSlot + kPfCodeSlot<NH> + w * kPfScaleWave;
+        const bool v0 = (vbits >> (2 * sl)) & 1u, v1 = (vbits >> (2 * sl + 1)) & 1u;
+        const int tok0 = (pg_first + 2 * i) * kPage;
+        const bool whole = v0 && v1 && tok0 + 2 * kPage <= tb;
+        // 256-wide heads: no mask-free copy (its register allocation spilled)
+        if (NH == 1 && whole && tok0 + 2 * kPage <= least)
+          pf_consume<HW, 0, Q8, NH>(acc, m, l, qh, ql, qexp, pl, sp, tok0, v0, v1, ta, tb, limit - 1, ta, true, g, n, sc, &vnorm);
+        else if (NH == 2 && whole)
+          pf_consume<HW, 1, Q8, NH>(acc, m, l, qh, ql, qexp, pl, sp, tok0, v0, v1, ta, tb, limit - 1, ta, true, g, n, sc, &vnorm);
+        else
+          pf_consume<HW, 2, Q8, NH>(acc, m, l, qh, ql, qexp, pl, sp, tok0, v0, v1, ta, tb, limit - 1, ta, true, g, n, sc, &vnorm);
+      }
+    }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int hh = 0; hh < HW; ++hh) {
+    const float lt = sum_xor16(sum_xor32(l[hh]));
+    if (lane < 16 && u0 + n < cols) {
+      int u = u0 + n;
+      asm volatile("" : "+v"(u));  // sequence and head again, not held through the loop
+      const RowOut o = row_out<D>(a, it, gr.first + u / per, kvh * a.rep + u % per * HW + hh);
+      o.ml[0] = m[hh];
+      o.ml[1] = lt;
+    }
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) {
+      const int u = u0 + 4 * g + ii;
+      if (u < cols) {
+        const RowOut o = row_out<D>(a, it, gr.first + u / per, kvh * a.rep + u % per * HW + hh);
+#pragma unroll
+        for (int nb = 0; nb < 8 * NH; ++nb) o.acc[16 * nb + n] = Q8 ? acc[hh][nb][ii] * vnorm : acc[hh][nb][ii];
+      }
+    }
+  }
+}
+
 // One partial row per query head of a group whose pages are split: wave per
 // (sequence, head), the splits in order.
 template <int D>
@@ -262,12 +465,27 @@ __global__ __launch_bounds__(kBlock) void prefix_merge_kernel(PrefixArgs a) {
   }
 }
 
+template <bool Q8>
+void launch_prefix_mfma(const PrefixArgs& a, int d, unsigned blocks, hipStream_t st) {
+  if (d == 256)
+    prefix_mfma_kernel<Q8, 2, 1><<<blocks, kWave * 8, 0, st>>>(a);
+  else if (a.rep > 1)
+    prefix_mfma_kernel<Q8, 1, 2><<<blocks, kWave * 8, 0, st>>>(a);
+  else
+    prefix_mfma_kernel<Q8, 1, 1><<<blocks, kWave * 8, 0, st>>>(a);
+}
+
 template <int DT>
 void launch_prefix_f32(const PrefixArgs& a, int d, unsigned blocks, hipStream_t st) {
   switch (d) {
-    case 64: prefix_f32_kernel<DT, 64><<<blocks, kBlock, 0, st>>>(a); break;
-    case 128: prefix_f32_kernel<DT, 128><<<blocks, kBlock, 0, st>>>(a); break;
-    default: prefix_f32_kernel<DT, 256><<<blocks, kBlock, 0, st>>>(a); break;
+    case 64: prefix_f32_kernel<DT, 64><<<blocks, kBlock, 0, st>>>(a); return;
+    default: break;
+  }
+  if constexpr (DT == LNSKV_DTYPE_F32) {
+    if (d == 128)
+      prefix_f32_kernel<DT, 128><<<blocks, kBlock, 0, st>>>(a);
+    else
+      prefix_f32_kernel<DT, 256><<<blocks, kBlock, 0, st>>>(a);
   }
 }
 
@@ -277,6 +495,7 @@ struct PrefixPlan {
   VarPlan own;            // the decode over the sequences' own pages
   int64_t units = 0;      // and its units at most
   int split_pages = 0;    // 0: nothing is shared
+  int tile_rows = 0;      // query rows of a work item
   int64_t items = 0;      // work items per kv head
   int64_t merge_rows = 0; // query heads of split groups
   int64_t part_rows = 0;  // partial rows
@@ -291,6 +510,8 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
     return fail(LNSKV_ERR_INVALID, "n_groups %d out of range [0, %d]", n_groups, LNSKV_PREFIX_MAX_GROUPS);
   if (n_groups > 0 && !groups) return fail(LNSKV_ERR_INVALID, "groups must be non-null");
   const int rep = n_heads / (int)c->n_kv_heads, d = (int)c->head_dim;
+  // the matrix-core kernel takes two heads of a sequence per column where it can
+  p->tile_rows = !var_mfma(c) ? kRowsTile : (d == 128 && rep > 1 ? 256 : 128);
   const int64_t all = (int64_t)max_kv_len / kPage + 1;
   int64_t own_pages = 0, most = 0, tiles = 0, max_shared = 0;  // summed over sequences; of one sequence
   int at = 0;
@@ -308,7 +529,7 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
     most = std::max(most, std::max<int64_t>(all - shared, 1));
     if (shared == 0) continue;
     p->g[p->n_groups++] = PrefixGroup{first, at, (int32_t)shared};
-    tiles += ceil_div(n * rep, kRowsTile);
+    tiles += ceil_div(n * rep, p->tile_rows);
     max_shared = std::max(max_shared, shared);
   }
   if (at < n_seq) most = all;
@@ -317,12 +538,13 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   if (int rc = plan_var<kPrefix>(c, n_seq, n_heads, p->units, most, p->n_groups == 0, &p->own)) return rc;
   p->ws_bytes = p->own.ws_bytes;
   if (p->n_groups == 0) return LNSKV_OK;
-  // splits of equal pages, about two items per compute unit
-  const int64_t want = std::max<int64_t>(1, 512 / (tiles * c->n_kv_heads));
+  // splits of equal pages, about one matrix-core item or two of the f32 kernel's per
+  // compute unit
+  const int64_t want = std::max<int64_t>(1, (var_mfma(c) ? 256 : 512) / (tiles * c->n_kv_heads));
   p->split_pages = (int)std::max<int64_t>(kSplitPages, (max_shared + want - 1) / want);
   for (int i = 0; i < p->n_groups; ++i) {
     const int64_t n = p->g[i].end - p->g[i].first, splits = ceil_div(p->g[i].pages, p->split_pages);
-    p->items += ceil_div((int)(n * rep), kRowsTile) * splits;
+    p->items += ceil_div((int)(n * rep), p->tile_rows) * splits;
     if (splits > 1) {
       p->merge_rows += n * n_heads;
       p->part_rows += n * n_heads * splits;
@@ -376,6 +598,12 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
     x.v_pages = a.v_pages;
     x.k_scales = a.k_scales;
     x.v_scales = a.v_scales;
+    x.pf.k_pages = a.k_pages;
+    x.pf.v_pages = a.v_pages;
+    x.pf.k_scales = a.k_scales;
+    x.pf.v_scales = a.v_scales;
+    x.pf.num_pages = c->num_pages;
+    x.pf.n_kv = a.n_kv;
     x.q = q;
     x.bt = bt;
     x.kv_len = kv_len;
@@ -396,8 +624,14 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
     const unsigned blocks = (unsigned)(p.items * a.n_kv);
     switch (c->dtype) {
       case LNSKV_DTYPE_F32: launch_prefix_f32<LNSKV_DTYPE_F32>(x, d, blocks, st); break;
-      case LNSKV_DTYPE_F16: launch_prefix_f32<LNSKV_DTYPE_F16>(x, d, blocks, st); break;
-      default: launch_prefix_f32<LNSKV_DTYPE_Q8A>(x, d, blocks, st); break;
+      case LNSKV_DTYPE_F16:
+        if (var_mfma(c)) launch_prefix_mfma<false>(x, d, blocks, st);
+        else launch_prefix_f32<LNSKV_DTYPE_F16>(x, d, blocks, st);
+        break;
+      default:
+        if (var_mfma(c)) launch_prefix_mfma<true>(x, d, blocks, st);
+        else launch_prefix_f32<LNSKV_DTYPE_Q8A>(x, d, blocks, st);
+        break;
     }
     if (int rc = hip_check("prefix kernel launch")) return rc;
     if (p.merge_rows > 0) {
