@@ -574,9 +574,9 @@ __device__ __forceinline__ void init_wave_state_q8(const DecodeArgs& a, const Pi
 // The end of a piece: sums over the lanes, then the normalised output rows
 // or the partial rows the piece leaves for a merge.
 // SC (Q8A pages): acc is in units of st.vnorm.
-template <int REP, bool SC = false, int NH = 1, int VAR = kPlain, class... SP>
+template <int REP, bool SC = false, int NH = 1>
 __device__ __forceinline__ void finish_piece(const DecodeArgs& a, WaveState<REP, NH>& st, int s, int kvh,
-                                             const PieceOut& po, int g, int n, const SP&... sp) {
+                                             const PieceOut& po, int g, int n) {
   constexpr int D = NH * kD;
   // Denominators: sum this head's lanes over the four 16-lane rows.
   st.l = sum_xor16(sum_xor32(st.l));
@@ -609,26 +609,6 @@ __device__ __forceinline__ void finish_piece(const DecodeArgs& a, WaveState<REP,
     lsel[ii] = (REP == 8 && g == 1) ? row_value<(4 + ii) % REP>(st.l) : row_value<ii>(st.l);
     msel[ii] = (REP == 8 && g == 1) ? row_value<(4 + ii) % REP>(st.m) : row_value<ii>(st.m);
   });
-  if constexpr (VAR == kPrefix) {
-    const PieceSeed& seed = only(sp...);
-    if (seed.seeded && (g == 0 || (REP == 8 && g == 1))) {
-      const int hb = REP == 8 ? 4 * g : 0;
-      // acc stays in units of vnorm (Q8A pages; 1 when no page set it)
-      if (SC && st.vnorm == 0.0f) st.vnorm = 1.0f;
-      const float unit = SC ? 1.0f / st.vnorm : 1.0f;
-      static_for<HL>([&](auto c) {
-        constexpr int ii = decltype(c)::value;
-        const size_t hrow = (size_t)s * a.n_heads + (size_t)kvh * REP + hb + ii;
-        const float ms = seed.ml[2 * hrow], M = fmaxf(msel[ii], ms);
-        const float wa = fast_exp2(msel[ii] - M), wb = fast_exp2(ms - M);
-        lsel[ii] = lsel[ii] * wa + seed.ml[2 * hrow + 1] * wb;
-        msel[ii] = M;
-#pragma unroll
-        for (int nb = 0; nb < 8 * NH; ++nb)
-          o[ii][nb] = o[ii][nb] * wa + seed.acc[hrow * D + 16 * nb + n] * (wb * unit);
-      });
-    }
-  }
   if (g == 0 || (REP == 8 && g == 1)) {
     const int hb = REP == 8 ? 4 * g : 0;
     static_for<HL>([&](auto c) {
@@ -677,7 +657,7 @@ __device__ __forceinline__ void run_piece(const DecodeArgs& a, lds_u8* vring, ld
                                           PieceLoads<REP, NH>& pl, bool tbl_ok, int s, int kvh, int ta, int tb,
                                           bool append, int pos, const PieceOut& po, lds_u8* rope_table,
                                           const SP&... sp) {
-  static_assert(!FUSED || VAR == kPlain, "the variants attend pages that hold every token");
+  static_assert(!FUSED || VAR == kPlain, "kSink attends pages that hold every token");
   const int lane = (int)(threadIdx.x & (kWave - 1));
   const int g = lane >> 4, n = lane & 15;
   constexpr int kRow = NH * kRowBytes;  // one (token, kv head) row of f16
@@ -880,7 +860,7 @@ __device__ __forceinline__ void run_piece(const DecodeArgs& a, lds_u8* vring, ld
   // the slots and the staged token are reused by the next piece
   __builtin_amdgcn_wave_barrier();
 
-  finish_piece<REP, false, NH, VAR>(a, st, s, kvh, po, g, n, sp...);
+  finish_piece<REP, false, NH>(a, st, s, kvh, po, g, n);
 }
 
 // ---------------------------------------------------------------------------
@@ -962,7 +942,7 @@ __device__ __forceinline__ void run_piece_q8(const DecodeArgs& a, lds_u8* vslot,
                                              PieceLoads<REP, NH>& pl, bool tbl_ok, int s, int kvh, int ta, int tb,
                                              bool append, int pos, const PieceOut& po,
                                              lds_u8* rope_table, const SP&... sp) {
-  static_assert(!FUSED || VAR == kPlain, "the variants attend pages that hold every token");
+  static_assert(!FUSED || VAR == kPlain, "kSink attends pages that hold every token");
   const int lane = (int)(threadIdx.x & (kWave - 1));
   const int g = lane >> 4, n = lane & 15;
   constexpr int kRowQ8 = NH * kD;  // one (token, kv head) row of int8 codes
@@ -1202,7 +1182,7 @@ __device__ __forceinline__ void run_piece_q8(const DecodeArgs& a, lds_u8* vslot,
     if (i + d < npg) step(i + d, pbuf[d % DEPTH], vld[d % DEPTH], false);
   wait_vmcnt<0>();  // stand-in pages of a piece with fewer than DEPTH pages
   __builtin_amdgcn_wave_barrier();
-  finish_piece<REP, true, NH, VAR>(a, st, s, kvh, po, g, n, sp...);
+  finish_piece<REP, true, NH>(a, st, s, kvh, po, g, n);
 }
 
 // Split-K schedule: block (kv head, partition, sequence) attends one
@@ -1265,7 +1245,6 @@ __device__ __forceinline__ SkSeq sk_fields(const DecodeArgs& a, int s, int n_seq
   // a length past what the grid or the table row can address marks the
   // sequence out of range: empty window, nothing stored
   L = L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : max(L, 0);
-  if constexpr (VAR == kPrefix) p0 = shared_pages(only(x...), s) * kPage;
   if constexpr (VAR == kSink) {  // pages counted from the first, without the gap
     const SinkSpan sp = sink_span(only(x...), L);
     q.L = L;
@@ -1286,16 +1265,6 @@ __device__ __forceinline__ SkSeq sk_fields(const DecodeArgs& a, int s, int n_seq
   q.cnt = q.np * a.n_kv;
   q.incl = 0;
   return q;
-}
-
-// Element i of the output row of a sequence with no pages of its own: what the
-// prefix gives it, or zero.
-template <int D>
-__device__ __forceinline__ float empty_window(const DecodeArgs& a, const VarArgs<kPrefix>& x, int p0, int s, int i) {
-  if (p0 == 0) return 0.0f;  // p0: min(shared tokens, length)
-  const size_t hrow = (size_t)s * a.n_heads + i / D;
-  const float l = x.seed_ml[2 * hrow + 1];
-  return gated(a, hrow * D + i % D, l > 0.0f ? x.seed_acc[hrow * D + i % D] / l : 0.0f);
 }
 
 // Three inclusive scans over the wave's lanes, their steps interleaved.
@@ -1423,20 +1392,16 @@ void decode_sk_kernel(DecodeArgs a, int n_seq, int n_waves, X... x) {
     po.final = i0 == 0 && i1 == np;
     po.pbase = ((size_t)wv * 2 + slot) * REP;
     po.pstride = 1;
-    if constexpr (VAR != kPlain) {
-      auto go = [&](const auto& sp, int te) {
-        if constexpr (Q8)
-          run_piece_q8<REP, DEPTH, FUSED, NH, ROPE, VAR>(a, (lds_u8*)vring_, (lds_u8*)newtok_, pl, true, s, kvh,
-                                                         max(p0, (pg0 + i0) * kPage), te, false, L - 1, po,
-                                                         (lds_u8*)rope_table_, sp);
-        else
-          run_piece<REP, FUSED, DEPTH, ROPE, NH, VAR>(a, (lds_u8*)vring_, (lds_u8*)newtok_, pl, true, s, kvh,
-                                                      max(p0, (pg0 + i0) * kPage), te, false, L - 1, po,
-                                                      (lds_u8*)rope_table_, sp);
-      };
-      // kSink: pages counted without the gap, tokens masked by the span
-      if constexpr (VAR == kSink) go(sink_span(x..., L), (pg0 + i1) * kPage);
-      else go(PieceSeed{i0 == 0 && p0 > 0, only(x...).seed_acc, only(x...).seed_ml}, min(L, (pg0 + i1) * kPage));
+    if constexpr (VAR == kSink) {  // pages counted without the gap, tokens masked by the span
+      const SinkSpan sp = sink_span(x..., L);
+      if constexpr (Q8)
+        run_piece_q8<REP, DEPTH, FUSED, NH, ROPE, VAR>(a, (lds_u8*)vring_, (lds_u8*)newtok_, pl, true, s, kvh,
+                                                       (pg0 + i0) * kPage, (pg0 + i1) * kPage, false, L - 1, po,
+                                                       (lds_u8*)rope_table_, sp);
+      else
+        run_piece<REP, FUSED, DEPTH, ROPE, NH, VAR>(a, (lds_u8*)vring_, (lds_u8*)newtok_, pl, true, s, kvh,
+                                                    (pg0 + i0) * kPage, (pg0 + i1) * kPage, false, L - 1, po,
+                                                    (lds_u8*)rope_table_, sp);
     } else if constexpr (Q8)
       run_piece_q8<REP, DEPTH, FUSED, NH, ROPE>(a, (lds_u8*)vring_, (lds_u8*)newtok_, pl, true, s, kvh,
                                                 max(p0, (pg0 + i0) * kPage), min(L, (pg0 + i1) * kPage),
@@ -1462,12 +1427,7 @@ __global__ __launch_bounds__(kBlock) void combine_sk_kernel(DecodeArgs a, int n_
   const int w = blockIdx.x, wv = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int4 d = a.sk_desc[w];
   for (int s = w; s < n_seq; s += n_waves) {  // block-uniform
-    if constexpr (VAR == kPrefix) {
-      const SkSeq e = sk_fields<FUSED, VAR>(a, s, n_seq, x...);
-      if (e.np == 0)
-        for (int i = threadIdx.x; i < a.n_heads * D; i += kBlock)
-          a.out[(size_t)s * a.n_heads * D + i] = empty_window<D>(a, x..., e.p0, s, i);
-    } else if (sk_fields<FUSED, VAR>(a, s, n_seq, x...).np == 0)
+    if (sk_fields<FUSED, VAR>(a, s, n_seq, x...).np == 0)
       for (int i = threadIdx.x; i < a.n_heads * D; i += kBlock) a.out[(size_t)s * a.n_heads * D + i] = 0.0f;
   }
   if (d.w == 0) return;
@@ -1684,20 +1644,16 @@ void decode_wg_kernel(DecodeArgs a, int n_seq, int n_wg, int n_cu, X... x) {
     po.pstride = 1;
     po.in_lds = true;
     po.lds = (lds_f32*)part_;
-    if constexpr (VAR != kPlain) {
-      auto go = [&](const auto& sp, int te) {
-        if constexpr (Q8)
-          run_piece_q8<REP, DEPTH, FUSED, NH, ROPE, VAR>(a, (lds_u8*)vring_[wi], (lds_u8*)newtok_[wi], pl, true, s, kvh,
-                                                         max(p0, (pg0 + i0) * kPage), te, false, L - 1, po,
-                                                         (lds_u8*)rope_table_[wi], sp);
-        else
-          run_piece<REP, FUSED, DEPTH, ROPE, NH, VAR>(a, (lds_u8*)vring_[wi], (lds_u8*)newtok_[wi], pl, true, s, kvh,
-                                                      max(p0, (pg0 + i0) * kPage), te, false, L - 1, po,
-                                                      (lds_u8*)rope_table_[wi], sp);
-      };
-      // kSink: pages counted without the gap, tokens masked by the span
-      if constexpr (VAR == kSink) go(sink_span(x..., L), (pg0 + i1) * kPage);
-      else go(PieceSeed{i0 == 0 && p0 > 0, only(x...).seed_acc, only(x...).seed_ml}, min(L, (pg0 + i1) * kPage));
+    if constexpr (VAR == kSink) {  // pages counted without the gap, tokens masked by the span
+      const SinkSpan sp = sink_span(x..., L);
+      if constexpr (Q8)
+        run_piece_q8<REP, DEPTH, FUSED, NH, ROPE, VAR>(a, (lds_u8*)vring_[wi], (lds_u8*)newtok_[wi], pl, true, s, kvh,
+                                                       (pg0 + i0) * kPage, (pg0 + i1) * kPage, false, L - 1, po,
+                                                       (lds_u8*)rope_table_[wi], sp);
+      else
+        run_piece<REP, FUSED, DEPTH, ROPE, NH, VAR>(a, (lds_u8*)vring_[wi], (lds_u8*)newtok_[wi], pl, true, s, kvh,
+                                                    (pg0 + i0) * kPage, (pg0 + i1) * kPage, false, L - 1, po,
+                                                    (lds_u8*)rope_table_[wi], sp);
     } else if constexpr (Q8)
       run_piece_q8<REP, DEPTH, FUSED, NH, ROPE>(a, (lds_u8*)vring_[wi], (lds_u8*)newtok_[wi], pl, true, s, kvh,
                                                 max(p0, (pg0 + i0) * kPage), min(L, (pg0 + i1) * kPage),
@@ -1913,12 +1869,7 @@ void decode_wg_kernel(DecodeArgs a, int n_seq, int n_wg, int n_cu, X... x) {
 
   // zero rows for the sequences with empty windows (wg, wg + G, ...)
   for (int s = wg; s < n_seq; s += n_wg) {  // block-uniform
-    if constexpr (VAR == kPrefix) {
-      const SkSeq e = sk_fields<FUSED, VAR>(a, s, n_seq, x...);
-      if (e.np == 0)
-        for (int i = threadIdx.x; i < a.n_heads * D; i += kWave * NW)
-          a.out[(size_t)s * a.n_heads * D + i] = empty_window<D>(a, x..., e.p0, s, i);
-    } else if (sk_fields<FUSED, VAR>(a, s, n_seq, x...).np == 0)
+    if (sk_fields<FUSED, VAR>(a, s, n_seq, x...).np == 0)
       for (int i = threadIdx.x; i < a.n_heads * D; i += kWave * NW) a.out[(size_t)s * a.n_heads * D + i] = 0.0f;
   }
 }

@@ -306,8 +306,12 @@ __global__ __launch_bounds__(kBlock) void decode_valu_kernel(DecodeArgs a, X... 
   if constexpr (VAR == kSink) sp = sink_span(only(x...), w.L);
   int tread_end = FUSED ? max(w.L - 1, 0) : w.L;  // newest token comes from registers
   if constexpr (VAR == kSink) tread_end = max(w.L - sp.gap * kPage, 0);  // ta, tb count without the gap
-  const int ta = max(w.p0, j * a.split);
-  const int tb = min(tread_end, (j + 1) * a.split);
+  int ta = max(w.p0, j * a.split);
+  int tb = min(tread_end, (j + 1) * a.split);
+  if constexpr (VAR == kPrefix) {  // partitions from the prefix's end on
+    ta = w.p0 + j * a.split;
+    tb = min(w.L, ta + a.split);
+  }
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int r = lane / G::LPR, c = lane % G::LPR;

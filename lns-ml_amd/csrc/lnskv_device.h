@@ -261,9 +261,8 @@ __device__ __forceinline__ float gated(const DecodeArgs& a, size_t idx, float v)
 //  kPlain   [p_start, L)
 //  kSink    the first n_sink tokens and the last `window` (0: all of them)
 //  kPrefix  [P, L), P the tokens that the sequence shares with its group; what
-//           the group's prefix gives its rows comes as a partial row per query
-//           head (numerator, running max, sum), merged where the segment's
-//           first page is
+//           the group's prefix gives its rows comes as partial rows (numerator,
+//           running max, sum) to merge (the generic kernel only)
 enum DecodeVariant { kPlain = 0, kSink = 1, kPrefix = 2 };
 template <int VAR> struct VarArgs {};
 template <> struct VarArgs<kSink> {
@@ -275,19 +274,28 @@ struct PrefixGroup {
   int32_t first, end, pages;
 };
 template <> struct VarArgs<kPrefix> {
-  const float* seed_acc;  // [n_seq][n_heads][D] numerators of the prefix
-  const float* seed_ml;   // [n_seq][n_heads][2] running max (log2 units) and sum
-  int32_t s0;             // the launch's first sequence
+  const float* part_acc;  // partial rows of the groups' prefixes: numerators,
+  const float* part_ml;   // running max (log2 units) and sum
+  int32_t split_pages;    // a group's pages are split every so many
   int32_t n_groups;
   PrefixGroup g[LNSKV_PREFIX_MAX_GROUPS];
 };
 
-// Shared pages of the launch's sequence s; 0 where it is in no group.
-__device__ __forceinline__ int shared_pages(const VarArgs<kPrefix>& x, int s) {
-  int p = 0;
-  for (int i = 0; i < x.n_groups; ++i)
-    if (s + x.s0 >= x.g[i].first && s + x.s0 < x.g[i].end) p = x.g[i].pages;
-  return p;
+// The shared pages of sequence s (0 where it is in no group) and its prefix's
+// partial rows: head h has rows base + h * splits .. + splits - 1.
+struct PrefixRows {
+  size_t base;
+  int splits, pages;
+};
+__device__ __forceinline__ PrefixRows prefix_rows(const VarArgs<kPrefix>& x, int s, int n_heads) {
+  size_t at = 0;
+  for (int i = 0; i < x.n_groups; ++i) {
+    const PrefixGroup g = x.g[i];
+    const int splits = (g.pages + x.split_pages - 1) / x.split_pages;
+    if (s >= g.first && s < g.end) return {at + (size_t)(s - g.first) * n_heads * splits, splits, g.pages};
+    at += (size_t)(g.end - g.first) * n_heads * splits;
+  }
+  return {0, 0, 0};
 }
 
 // kSink: the attended tokens of a sequence are t < n_sink and p0 <= t < L.
@@ -315,15 +323,9 @@ __device__ __forceinline__ bool span_sees(int t, const SinkSpan& sp) { return si
 __device__ __forceinline__ bool span_sees(int) { return true; }
 // The kernels pass what belongs to a variant as a parameter pack that is empty
 // for kPlain, so that the plain kernels compile to what they are without it:
-// the arguments of a call (VarArgs), the span of a sequence (SinkSpan), the
-// seed rows of a piece (PieceSeed).
+// the arguments of a call (VarArgs), the span of a sequence (SinkSpan).
 template <class X>
 __device__ __forceinline__ const X& only(const X& x) { return x; }
-struct PieceSeed {  // kPrefix: the rows that the piece which starts a segment merges
-  bool seeded;
-  const float* acc;
-  const float* ml;
-};
 
 struct SeqWindow {
   int L;       // kv_len; 0 when it is past what the grid or the table row can address
@@ -349,7 +351,14 @@ __device__ __forceinline__ SeqWindow seq_window(const DecodeArgs& a, int s, cons
     return w;
   }
   int p0 = a.p_start ? a.p_start[s] : a.p_start_scalar;
-  if constexpr (VAR == kPrefix) p0 = shared_pages(only(x...), s) * kPage;
+  if constexpr (VAR == kPrefix) {  // partitions from the prefix's end on
+    p0 = min(prefix_rows(only(x...), s, a.n_heads).pages * kPage, L);
+    w.L = L;
+    w.p0 = p0;
+    w.jf = 0;
+    w.nparts = max(1, (L - p0 + a.split - 1) / a.split);
+    return w;
+  }
   p0 = min(max(p0, 0), L);
   int lo = p0;
   if (FUSED && L > 0) lo = min(lo, L - 1);
@@ -383,7 +392,7 @@ struct EpilogueLds {
   float l[kWavesPerBlock][REP];
 };
 
-// kPrefix: the first partition's block merges the prefix's row as well.
+// kPrefix: the first partition's block merges the prefix's rows as well.
 template <int REP, int D, int VAR = kPlain, class... X>
 __device__ __forceinline__ void finish_block(const DecodeArgs& a, EpilogueLds<REP, D>& sm, const SeqWindow& w,
                                              int s, int kvh, int part, const X&... x) {
@@ -403,13 +412,17 @@ __device__ __forceinline__ void finish_block(const DecodeArgs& a, EpilogueLds<RE
     }
     const size_t hrow = (size_t)s * a.n_heads + h0 + h;
     if constexpr (VAR == kPrefix) {
-      if (part == 0 && w.p0 > 0) {  // block-uniform
-        const VarArgs<kPrefix>& pf = only(x...);
-        const float ms = pf.seed_ml[2 * hrow], Mn = fmaxf(M, ms);
-        const float wa = fast_exp2(M - Mn), wb = fast_exp2(ms - Mn);
-        A = A * wa + pf.seed_acc[hrow * D + i] * wb;
-        Ls = Ls * wa + pf.seed_ml[2 * hrow + 1] * wb;
-        M = Mn;
+      if (part == 0) {  // block-uniform
+        const VarArgs<kPrefix>& px = only(x...);
+        const PrefixRows pr = prefix_rows(px, s, a.n_heads);
+        const size_t r0 = pr.base + (size_t)(h0 + h) * pr.splits;
+        for (int j = 0; j < pr.splits; ++j) {
+          const float ms = px.part_ml[2 * (r0 + j)], ls = px.part_ml[2 * (r0 + j) + 1], Mn = fmaxf(M, ms);
+          const float wa = fast_exp2(M - Mn), wb = fast_exp2(ms - Mn);
+          A = A * wa + px.part_acc[(r0 + j) * D + i] * wb;
+          Ls = Ls * wa + ls * wb;
+          M = Mn;
+        }
       }
     }
     if (single) {

@@ -7,10 +7,14 @@
 //   out = (2^(m1 - M) A1 + 2^(m2 - M) A2) / (2^(m1 - M) l1 + 2^(m2 - M) l2).
 // 1. prefix kernels: work item = (group, tile of the group's query rows, split of its
 //    pages, kv head).  A row is one query head of one sequence; all rows of a
-//    tile multiply the same K and V.  Each item leaves a partial row (A, m, l).
-// 2. merge kernel, when some group's pages are split: one partial row per query head.
-// 3. the decode kernels' kPrefix variant over [P, L): the piece that starts a
-//    sequence's segment merges its prefix row.
+//    tile multiply the same K and V.  Each item leaves a partial row (A, m, l)
+//    per query row.
+// 2. own kernel (f16 and Q8A pages, 128- and 256-wide heads; the generic decode
+//    kernel elsewhere): work item = (sequence, kv head, share of its own pages);
+//    a sequence with one share merges the prefix's rows and writes its output.
+// 3. join kernel, where sequences may have several shares: their rows and the
+//    prefix's into the output.
+#include "lnskv_decode_mfma.h"
 #include "lnskv_decode_var.h"
 #include "lnskv_prefill.h"
 
@@ -18,7 +22,10 @@ namespace lnskv {
 namespace {
 
 constexpr int kRowsTile = 64;   // query rows per tile of the f32 kernel: four waves of 16
-constexpr int kSplitPages = 4;  // fewest pages of a split
+constexpr int kSplitPages = 16;    // fewest pages of a split, matrix-core kernel
+constexpr int kSplitPagesF32 = 2;  // f32 kernel
+constexpr int kSharePages = 64;    // most pages of a share of a sequence's own
+constexpr int kShareMin = 8;
 
 struct PrefixArgs {
   PrefillArgs pf;  // the pools, for the prefill kernel's page pipeline
@@ -29,9 +36,7 @@ struct PrefixArgs {
   const float* q;         // [n_seq][n_heads][D]
   const uint32_t* bt;     // [n_seq][bt_stride]
   const int32_t* kv_len;  // [n_seq]
-  float* seed_acc;        // [n_seq][n_heads][D]: the groups' result
-  float* seed_ml;         // [n_seq][n_heads][2]
-  float* part_acc;        // partial rows of the groups with more than one split
+  float* part_acc;        // partial rows [group][its sequence][head][split]
   float* part_ml;
   int32_t bt_stride;
   int32_t n_kv;
@@ -66,21 +71,18 @@ __device__ __forceinline__ PrefixItem prefix_item(const PrefixArgs& a, int i, in
       return it;
     }
     i -= tiles * splits;
-    if (splits > 1) it.part0 += (size_t)rows * a.n_kv * splits;
+    it.part0 += (size_t)rows * a.n_kv * splits;
   }
   return it;
 }
 
-// Where row (sequence s, query head h) of an item goes: its seed row, or its
-// partial row [row of the group][split].
+// Where row (sequence s, query head h) of an item goes.
 struct RowOut {
   float* acc;
   float* ml;
 };
 template <int D>
 __device__ __forceinline__ RowOut row_out(const PrefixArgs& a, const PrefixItem& it, int s, int h) {
-  const size_t hrow = (size_t)s * a.n_heads + h;
-  if (it.splits == 1) return {a.seed_acc + hrow * D, a.seed_ml + 2 * hrow};
   const size_t r = it.part0 + ((size_t)(s - a.g[it.group].first) * a.n_heads + h) * it.splits + it.split;
   return {a.part_acc + r * D, a.part_ml + 2 * r};
 }
@@ -435,33 +437,157 @@ __global__ __launch_bounds__(kWave * 8) void prefix_mfma_kernel(PrefixArgs a) {
   }
 }
 
-// One partial row per query head of a group whose pages are split: wave per
-// (sequence, head), the splits in order.
+// ---------------------------------------------------------------------------
+// The sequences' own pages [P, L).  A workgroup takes one share (at most
+// share_pages pages) of one (sequence, kv head); its four waves split the share
+// and stream their pages as the decode kernels do, each by itself (K to registers,
+// V through an LDS ring, two pages in flight), leave partial rows in LDS, and
+// merge them head by head.  No workgroup depends on another.
+struct OwnArgs {
+  VarArgs<kPrefix> prefix;
+  float* own_acc;  // [n_seq][n_heads][shares][D], where a sequence has several shares
+  float* own_ml;
+  int32_t n_seq;
+  int32_t shares;  // of a sequence at most
+  int32_t share_pages;
+};
+
+// Pages of sequence s past its prefix, and how many shares they make.
+struct OwnSpan {
+  int L, p0, pages, shares;
+  PrefixRows prefix;
+};
+__device__ __forceinline__ OwnSpan own_span(const DecodeArgs& a, const OwnArgs& x, int s) {
+  OwnSpan o;
+  int L = a.kv_len[s];
+  o.L = L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : max(L, 0);
+  o.prefix = prefix_rows(x.prefix, s, a.n_heads);
+  o.p0 = min(o.prefix.pages * kPage, o.L);
+  o.pages = o.L > o.p0 ? (o.L - 1) / kPage - o.p0 / kPage + 1 : 0;
+  o.shares = max(1, ceil_div(o.pages, x.share_pages));
+  return o;
+}
+
+// Merges rows [r0, r0 + n) of (acc, ml) into (M, Ls, A): lane l holds columns
+// l + 64 c; eight rows' loads in flight.
 template <int D>
-__global__ __launch_bounds__(kBlock) void prefix_merge_kernel(PrefixArgs a) {
+__device__ __forceinline__ void merge_rows(const float* acc, const float* ml, size_t r0, int n, float& M, float& Ls,
+                                           float (&A)[D / kWave]) {
   constexpr int C = D / kWave;
-  int i = (int)blockIdx.x * kWavesPerBlock + (int)(threadIdx.x / kWave);
-  const int lane = threadIdx.x % kWave;
-  size_t part0 = 0;
-  for (int g = 0; g < a.n_groups; ++g) {
-    const int rows = (a.g[g].end - a.g[g].first) * a.n_heads, splits = ceil_div(a.g[g].pages, a.split_pages);
-    if (splits <= 1) continue;
-    if (i < rows) {  // wave-uniform
-      const size_t base = part0 + (size_t)i * splits;
-      float M, Ls, A[C];
-      merge_wave<D, 1, 8>(reinterpret_cast<const float2*>(a.part_ml), a.part_acc, 0, splits,
-                          [=](int j) { return base + (size_t)j; }, M, Ls, A);
-      const size_t hrow = (size_t)a.g[g].first * a.n_heads + i;
+  float m2, l2, a2[C];
+  merge_wave<D, 1, 8>(reinterpret_cast<const float2*>(ml), acc, 0, n, [=](int j) { return r0 + (size_t)j; }, m2, l2, a2);
+  const float Mn = fmaxf(M, m2), wa = fast_exp2(M - Mn), wb = fast_exp2(m2 - Mn);
+  M = Mn;
+  Ls = Ls * wa + l2 * wb;
 #pragma unroll
-      for (int c = 0; c < C; ++c) a.seed_acc[hrow * D + c * kWave + lane] = A[c];
-      if (lane == 0) {
-        a.seed_ml[2 * hrow] = M;
-        a.seed_ml[2 * hrow + 1] = Ls;
-      }
-      return;
+  for (int c = 0; c < C; ++c) A[c] = A[c] * wa + a2[c] * wb;
+}
+
+constexpr int kOwnWaves = 4;
+
+template <int REP, bool Q8, int NH>
+__global__ __launch_bounds__(kWave* kOwnWaves) __attribute__((amdgpu_waves_per_eu(NH == 1 ? 2 : 1)))
+void prefix_own_kernel(DecodeArgs a, OwnArgs x) {
+  constexpr int NW = kOwnWaves, D = NH * kD, C = D / kWave, kRow = D + 2;
+  constexpr int kSlots = Q8 ? 1 : 2;
+  typedef __attribute__((address_space(3))) float lds_f32;
+  __shared__ __attribute__((aligned(16))) uint8_t vring_[NW][kSlots * NH * kVSlot];
+  __shared__ __attribute__((aligned(16))) float part_[NW * REP * kRow];
+  const int wi = (int)(threadIdx.x / kWave), lane = (int)(threadIdx.x % kWave);
+  // share slowest: the first shares, which every sequence has, start first
+  const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
+  const int s = (int)(blockIdx.x / (unsigned)a.n_kv % (unsigned)x.n_seq);
+  const int share = (int)(blockIdx.x / (unsigned)a.n_kv / (unsigned)x.n_seq);
+  const OwnSpan o = own_span(a, x, s);
+  if (share >= o.shares) return;  // block-uniform
+  const int lo = (int)((int64_t)o.pages * share / o.shares), hi = (int)((int64_t)o.pages * (share + 1) / o.shares);
+  // wave w: pages [lo + w per, lo + (w + 1) per) of the sequence's own
+  const int per = ceil_div(hi - lo, NW);
+  const int i0 = min(hi, lo + wi * per), i1 = min(hi, i0 + per);
+  if (i0 < i1) {
+    const int pg0 = o.p0 / kPage;
+    PieceLoads<REP, NH> pl;
+    piece_loads<REP, false, false, Q8, NH>(a, s, kvh, pg0 + i0, pl);
+    PieceOut po;
+    po.final = false;
+    po.pbase = (size_t)wi * REP;
+    po.pstride = 1;
+    po.in_lds = true;
+    po.lds = (lds_f32*)part_;
+    if constexpr (Q8)
+      run_piece_q8<REP, 2, false, NH, false>(a, (lds_u8*)vring_[wi], (lds_u8*)vring_[wi], pl, true, s, kvh,
+                                             (pg0 + i0) * kPage, min(o.L, (pg0 + i1) * kPage), false, o.L - 1, po, nullptr);
+    else
+      run_piece<REP, false, 2, false, NH>(a, (lds_u8*)vring_[wi], (lds_u8*)vring_[wi], pl, true, s, kvh,
+                                          (pg0 + i0) * kPage, min(o.L, (pg0 + i1) * kPage), false, o.L - 1, po, nullptr);
+  }
+  __syncthreads();
+  const int nw = hi > lo ? ceil_div(hi - lo, per) : 0;  // waves that left rows
+  for (int h = wi; h < REP; h += NW) {  // wave-uniform
+    const size_t hrow = (size_t)s * a.n_heads + (size_t)kvh * REP + h;
+    float M = kMInit, Ls = 0.0f, A[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) A[c] = 0.0f;
+    for (int w = 0; w < nw; ++w) {
+      const lds_f32* row = (const lds_f32*)part_ + ((size_t)w * REP + h) * kRow;
+      const float m = row[D], Mn = fmaxf(M, m);
+      const float wa = fast_exp2(M - Mn), wb = fast_exp2(m - Mn);
+      Ls = Ls * wa + row[D + 1] * wb;
+#pragma unroll
+      for (int c = 0; c < C; ++c) A[c] = A[c] * wa + row[lane + c * kWave] * wb;
+      M = Mn;
     }
-    i -= rows;
-    part0 += (size_t)rows * splits;
+    if (o.shares == 1) {
+      merge_rows<D>(x.prefix.part_acc, x.prefix.part_ml, o.prefix.base + (size_t)(kvh * REP + h) * o.prefix.splits,
+                    o.prefix.splits, M, Ls, A);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const size_t i = hrow * D + c * kWave + lane;
+        a.out[i] = gated(a, i, Ls > 0.0f ? A[c] / Ls : 0.0f);
+      }
+    } else {
+      const size_t r = hrow * x.shares + share;
+#pragma unroll
+      for (int c = 0; c < C; ++c) x.own_acc[r * D + c * kWave + lane] = A[c];
+      if (lane == 0) {
+        x.own_ml[2 * r] = M;
+        x.own_ml[2 * r + 1] = Ls;
+      }
+    }
+  }
+}
+
+// The outputs of the sequences with several shares: wave per (sequence, head).
+template <int D>
+__global__ __launch_bounds__(kBlock) void prefix_join_kernel(DecodeArgs a, OwnArgs x) {
+  constexpr int C = D / kWave;
+  const int64_t i = (int64_t)blockIdx.x * kWavesPerBlock + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  if (i >= (int64_t)x.n_seq * a.n_heads) return;
+  const int s = __builtin_amdgcn_readfirstlane((int)(i / a.n_heads));
+  const int h = __builtin_amdgcn_readfirstlane((int)(i - (int64_t)s * a.n_heads));
+  const OwnSpan o = own_span(a, x, s);
+  if (o.shares == 1) return;
+  float M = kMInit, Ls = 0.0f, A[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) A[c] = 0.0f;
+  merge_rows<D>(x.own_acc, x.own_ml, (size_t)i * x.shares, o.shares, M, Ls, A);
+  merge_rows<D>(x.prefix.part_acc, x.prefix.part_ml, o.prefix.base + (size_t)h * o.prefix.splits, o.prefix.splits, M,
+                Ls, A);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const size_t e = (size_t)i * D + c * kWave + lane;
+    a.out[e] = gated(a, e, Ls > 0.0f ? A[c] / Ls : 0.0f);
+  }
+}
+
+template <bool Q8, int NH>
+void launch_own_rep(const DecodeArgs& a, const OwnArgs& x, int rep, unsigned blocks, hipStream_t st) {
+  switch (rep) {
+    case 1: prefix_own_kernel<1, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
+    case 2: prefix_own_kernel<2, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
+    case 4: prefix_own_kernel<4, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
+    default: prefix_own_kernel<8, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
   }
 }
 
@@ -492,14 +618,14 @@ void launch_prefix_f32(const PrefixArgs& a, int d, unsigned blocks, hipStream_t 
 // ---------------------------------------------------------------------------
 // The host's view of a call.
 struct PrefixPlan {
-  VarPlan own;            // the decode over the sequences' own pages
-  int64_t units = 0;      // and its units at most
-  int split_pages = 0;    // 0: nothing is shared
+  VarPlan own;            // the generic kernel over the sequences' own pages
+  int shares = 0;         // own kernel: shares of a sequence at most (0: the generic kernel)
+  int share_pages = 0;
+  int split_pages = 1;
   int tile_rows = 0;      // query rows of a work item
   int64_t items = 0;      // work items per kv head
-  int64_t merge_rows = 0; // query heads of split groups
-  int64_t part_rows = 0;  // partial rows
-  size_t seed_at = 0, part_at = 0, ws_bytes = 0;
+  int64_t part_rows = 0;  // partial rows of the prefixes
+  size_t own_at = 0, part_at = 0, ws_bytes = 0;
   int n_groups = 0;
   PrefixGroup g[LNSKV_PREFIX_MAX_GROUPS];
 };
@@ -534,26 +660,33 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   }
   if (at < n_seq) most = all;
   own_pages += (n_seq - at) * all;
-  p->units = own_pages * c->n_kv_heads;
-  if (int rc = plan_var<kPrefix>(c, n_seq, n_heads, p->units, most, p->n_groups == 0, &p->own)) return rc;
-  p->ws_bytes = p->own.ws_bytes;
+  const size_t row = ((size_t)d + 2) * sizeof(float);
+  if (var_mfma(c)) {
+    // shares of at most kSharePages pages, fewer where that leaves compute units idle
+    const int64_t units = own_pages * c->n_kv_heads;
+    p->share_pages = (int)std::min<int64_t>(kSharePages, std::max<int64_t>(kShareMin, (units + 511) / 512));
+    p->shares = (int)std::max<int64_t>(1, (most + p->share_pages - 1) / p->share_pages);
+    if ((int64_t)p->shares * n_seq * c->n_kv_heads > INT32_MAX)
+      return fail(LNSKV_ERR_UNSUPPORTED, "a batch of more than 2^31 shares");
+    p->own_at = kWsHeaderBytes;
+    p->ws_bytes = p->shares > 1 ? kWsHeaderBytes + (size_t)p->shares * n_seq * n_heads * row : 0;
+  } else {
+    if (int rc = plan_generic(c, n_seq, n_heads, most, &p->own)) return rc;
+    p->ws_bytes = p->own.ws_bytes;
+  }
   if (p->n_groups == 0) return LNSKV_OK;
   // splits of equal pages, about one matrix-core item or two of the f32 kernel's per
   // compute unit
   const int64_t want = std::max<int64_t>(1, (var_mfma(c) ? 256 : 512) / (tiles * c->n_kv_heads));
-  p->split_pages = (int)std::max<int64_t>(kSplitPages, (max_shared + want - 1) / want);
+  p->split_pages = (int)std::max<int64_t>(var_mfma(c) ? kSplitPages : kSplitPagesF32, (max_shared + want - 1) / want);
   for (int i = 0; i < p->n_groups; ++i) {
     const int64_t n = p->g[i].end - p->g[i].first, splits = ceil_div(p->g[i].pages, p->split_pages);
     p->items += ceil_div((int)(n * rep), p->tile_rows) * splits;
-    if (splits > 1) {
-      p->merge_rows += n * n_heads;
-      p->part_rows += n * n_heads * splits;
-    }
+    p->part_rows += n * n_heads * splits;
   }
-  if (p->items * c->n_kv_heads > INT32_MAX) return fail(LNSKV_ERR_INVALID, "too many row tiles");
-  p->seed_at = (std::max(p->ws_bytes, kWsHeaderBytes) + 255) & ~(size_t)255;
-  p->part_at = p->seed_at + (((size_t)n_seq * n_heads * (d + 2) * sizeof(float) + 255) & ~(size_t)255);
-  p->ws_bytes = p->part_at + (size_t)p->part_rows * (d + 2) * sizeof(float);
+  if (p->items * c->n_kv_heads > INT32_MAX) return fail(LNSKV_ERR_UNSUPPORTED, "too many row tiles");
+  p->part_at = (std::max(p->ws_bytes, kWsHeaderBytes) + 255) & ~(size_t)255;
+  p->ws_bytes = p->part_at + (size_t)p->part_rows * row;
   return LNSKV_OK;
 }
 
@@ -590,25 +723,29 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
   if (int rc = var_workspace(&ws, ws_bytes, p.ws_bytes, st)) return rc;
   const DecodeArgs a = var_args(c, q, out, gate, bt, bt_stride, kv_len, n_heads, max_kv_len, scale, p.own, stream);
   const int d = (int)c->head_dim;
-  float *seed_acc = nullptr, *seed_ml = nullptr;
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  OwnArgs o{};
+  o.n_seq = n_seq;
+  o.shares = p.shares;
+  o.share_pages = p.share_pages;
+  o.prefix.n_groups = p.n_groups;
+  o.prefix.split_pages = p.split_pages;
+  std::copy(p.g, p.g + p.n_groups, o.prefix.g);
   if (p.n_groups > 0) {
-    uint8_t* base = static_cast<uint8_t*>(ws);
     PrefixArgs x{};
-    x.k_pages = a.k_pages;
-    x.v_pages = a.v_pages;
-    x.k_scales = a.k_scales;
-    x.v_scales = a.v_scales;
     x.pf.k_pages = a.k_pages;
     x.pf.v_pages = a.v_pages;
     x.pf.k_scales = a.k_scales;
     x.pf.v_scales = a.v_scales;
     x.pf.num_pages = c->num_pages;
     x.pf.n_kv = a.n_kv;
+    x.k_pages = a.k_pages;
+    x.v_pages = a.v_pages;
+    x.k_scales = a.k_scales;
+    x.v_scales = a.v_scales;
     x.q = q;
     x.bt = bt;
     x.kv_len = kv_len;
-    x.seed_acc = seed_acc = reinterpret_cast<float*>(base + p.seed_at);
-    x.seed_ml = seed_ml = seed_acc + (size_t)n_seq * n_heads * d;
     x.part_acc = reinterpret_cast<float*>(base + p.part_at);
     x.part_ml = x.part_acc + (size_t)p.part_rows * d;
     x.bt_stride = bt_stride;
@@ -621,6 +758,8 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
     x.num_pages = c->num_pages;
     x.scale_log2 = a.scale_log2;
     std::copy(p.g, p.g + p.n_groups, x.g);
+    o.prefix.part_acc = x.part_acc;
+    o.prefix.part_ml = x.part_ml;
     const unsigned blocks = (unsigned)(p.items * a.n_kv);
     switch (c->dtype) {
       case LNSKV_DTYPE_F32: launch_prefix_f32<LNSKV_DTYPE_F32>(x, d, blocks, st); break;
@@ -634,26 +773,29 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
         break;
     }
     if (int rc = hip_check("prefix kernel launch")) return rc;
-    if (p.merge_rows > 0) {
-      const unsigned mb = (unsigned)((p.merge_rows + kWavesPerBlock - 1) / kWavesPerBlock);
-      switch (d) {
-        case 64: prefix_merge_kernel<64><<<mb, kBlock, 0, st>>>(x); break;
-        case 128: prefix_merge_kernel<128><<<mb, kBlock, 0, st>>>(x); break;
-        default: prefix_merge_kernel<256><<<mb, kBlock, 0, st>>>(x); break;
-      }
-      if (int rc = hip_check("prefix merge kernel launch")) return rc;
-    }
   }
-  return launch_plan<kPrefix>(c, a, p.own, p.units, n_seq, ws, st, [&](int s0) {
-    VarArgs<kPrefix> x{};
-    const size_t r = (size_t)s0 * n_heads;
-    x.seed_acc = seed_acc ? seed_acc + r * d : nullptr;
-    x.seed_ml = seed_ml ? seed_ml + 2 * r : nullptr;
-    x.s0 = s0;
-    x.n_groups = p.n_groups;
-    std::copy(p.g, p.g + p.n_groups, x.g);
-    return x;
-  });
+  if (p.shares == 0) return launch_generic<kPrefix>(c, a, p.own, n_seq, ws, o.prefix, st);
+  if (p.shares > 1) {
+    o.own_acc = reinterpret_cast<float*>(base + p.own_at);
+    o.own_ml = o.own_acc + (size_t)p.shares * n_seq * n_heads * d;
+  }
+  const unsigned blocks = (unsigned)((int64_t)p.shares * n_seq * a.n_kv);
+  const int rep = n_heads / a.n_kv;
+  if (c->dtype == LNSKV_DTYPE_Q8A) {
+    if (d == 256) launch_own_rep<true, 2>(a, o, rep, blocks, st);
+    else launch_own_rep<true, 1>(a, o, rep, blocks, st);
+  } else {
+    if (d == 256) launch_own_rep<false, 2>(a, o, rep, blocks, st);
+    else launch_own_rep<false, 1>(a, o, rep, blocks, st);
+  }
+  if (int rc = hip_check("own pages kernel launch")) return rc;
+  if (p.shares > 1) {
+    const unsigned jb = (unsigned)(((int64_t)n_seq * n_heads + kWavesPerBlock - 1) / kWavesPerBlock);
+    if (d == 256) prefix_join_kernel<256><<<jb, kBlock, 0, st>>>(a, o);
+    else prefix_join_kernel<128><<<jb, kBlock, 0, st>>>(a, o);
+    return hip_check("prefix join kernel launch");
+  }
+  return LNSKV_OK;
 }
 
 }  // extern "C"
