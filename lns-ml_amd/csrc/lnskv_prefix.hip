@@ -22,7 +22,7 @@ namespace lnskv {
 namespace {
 
 constexpr int kRowsTile = 64;   // query rows per tile of the f32 kernel: four waves of 16
-constexpr int kSplitPages = 16;    // fewest pages of a split, matrix-core kernel
+constexpr int kSplitPages = 8;     // fewest pages of a split, matrix-core kernel
 constexpr int kSplitPagesF32 = 2;  // f32 kernel
 constexpr int kSharePages = 64;    // most pages of a share of a sequence's own
 constexpr int kShareMin = 8;
@@ -592,10 +592,10 @@ void launch_own_rep(const DecodeArgs& a, const OwnArgs& x, int rep, unsigned blo
 }
 
 template <bool Q8>
-void launch_prefix_mfma(const PrefixArgs& a, int d, unsigned blocks, hipStream_t st) {
+void launch_prefix_mfma(const PrefixArgs& a, int d, int tile_rows, unsigned blocks, hipStream_t st) {
   if (d == 256)
     prefix_mfma_kernel<Q8, 2, 1><<<blocks, kWave * 8, 0, st>>>(a);
-  else if (a.rep > 1)
+  else if (tile_rows == 256)
     prefix_mfma_kernel<Q8, 1, 2><<<blocks, kWave * 8, 0, st>>>(a);
   else
     prefix_mfma_kernel<Q8, 1, 1><<<blocks, kWave * 8, 0, st>>>(a);
@@ -636,8 +636,11 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
     return fail(LNSKV_ERR_INVALID, "n_groups %d out of range [0, %d]", n_groups, LNSKV_PREFIX_MAX_GROUPS);
   if (n_groups > 0 && !groups) return fail(LNSKV_ERR_INVALID, "groups must be non-null");
   const int rep = n_heads / (int)c->n_kv_heads, d = (int)c->head_dim;
-  // the matrix-core kernel takes two heads of a sequence per column where it can
-  p->tile_rows = !var_mfma(c) ? kRowsTile : (d == 128 && rep > 1 ? 256 : 128);
+  // the matrix-core kernel takes two heads of a sequence per column where some
+  // group has more than 128 rows
+  int most_rows = 0;
+  for (int i = 0; i < n_groups; ++i) most_rows = std::max(most_rows, std::min(groups[3 * i + 1], n_seq) * rep);
+  p->tile_rows = !var_mfma(c) ? kRowsTile : (d == 128 && rep > 1 && most_rows > 128 ? 256 : 128);
   const int64_t all = (int64_t)max_kv_len / kPage + 1;
   int64_t own_pages = 0, most = 0, tiles = 0, max_shared = 0;  // summed over sequences; of one sequence
   int at = 0;
@@ -664,7 +667,9 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   if (var_mfma(c)) {
     // shares of at most kSharePages pages, fewer where that leaves compute units idle
     const int64_t units = own_pages * c->n_kv_heads;
-    p->share_pages = (int)std::min<int64_t>(kSharePages, std::max<int64_t>(kShareMin, (units + 511) / 512));
+    p->share_pages = n_seq * (int64_t)c->n_kv_heads >= 256
+                         ? kSharePages
+                         : (int)std::min<int64_t>(kSharePages, std::max<int64_t>(kShareMin, (units + 511) / 512));
     p->shares = (int)std::max<int64_t>(1, (most + p->share_pages - 1) / p->share_pages);
     if ((int64_t)p->shares * n_seq * c->n_kv_heads > INT32_MAX)
       return fail(LNSKV_ERR_UNSUPPORTED, "a batch of more than 2^31 shares");
@@ -764,11 +769,11 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
     switch (c->dtype) {
       case LNSKV_DTYPE_F32: launch_prefix_f32<LNSKV_DTYPE_F32>(x, d, blocks, st); break;
       case LNSKV_DTYPE_F16:
-        if (var_mfma(c)) launch_prefix_mfma<false>(x, d, blocks, st);
+        if (var_mfma(c)) launch_prefix_mfma<false>(x, d, p.tile_rows, blocks, st);
         else launch_prefix_f32<LNSKV_DTYPE_F16>(x, d, blocks, st);
         break;
       default:
-        if (var_mfma(c)) launch_prefix_mfma<true>(x, d, blocks, st);
+        if (var_mfma(c)) launch_prefix_mfma<true>(x, d, p.tile_rows, blocks, st);
         else launch_prefix_f32<LNSKV_DTYPE_Q8A>(x, d, blocks, st);
         break;
     }

@@ -20,13 +20,17 @@ def _ptr(t: torch.Tensor | None) -> C.c_void_p:
     return C.c_void_p(t.data_ptr() if t is not None else 0)
 
 
+def _address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def _stream(device: torch.device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 class _on:
-    """Makes a device current for a call (streams and workspaces are per device);
-    nothing when it is already."""
+    """Makes a device current for a call (streams and workspaces are per device) and
+    yields its current stream; does nothing else where it is current already."""
 
     __slots__ = ("index", "before")
 
@@ -34,12 +38,11 @@ class _on:
         self.index = device.index
 
     def __enter__(self):
-        self.before = None
-        if self.index is not None:
-            now = torch.cuda.current_device()
-            if now != self.index:
-                self.before = now
-                torch.cuda.set_device(self.index)
+        now = torch._C._cuda_getDevice()
+        self.before = now if now != self.index else None
+        if self.before is not None:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.before is not None:
@@ -307,11 +310,11 @@ class PagedKV:
             _need(q_out, "q_out", torch.float32, q.numel(), dev)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        with _on(dev):
-            check(lib().lnskv_mrope_append(self._c, rope._c, rope._sections, rope.n_axes, rope.interleaved, _ptr(q),
-                                           _ptr(q_out), n_heads, _ptr(k_new), _ptr(v_new), _ptr(axis_pos),
-                                           _ptr(tok_seq), _ptr(tok_pos), n_tok, _ptr(tables), stride,
-                                           int(tables.shape[0]), _stream(dev)))
+        with _on(dev) as stream:
+            check(lib().lnskv_mrope_append(self._c, rope._c, rope._sections, rope.n_axes, rope.interleaved, _address(q),
+                                           _address(q_out), n_heads, k_new.data_ptr(), v_new.data_ptr(), axis_pos.data_ptr(),
+                                           tok_seq.data_ptr(), tok_pos.data_ptr(), n_tok, tables.data_ptr(), stride,
+                                           int(tables.shape[0]), stream))
         return q_out
 
     def sink_workspace_size(self, n_seq: int, n_heads: int, max_kv_len: int, window: int, n_sink: int) -> int:
@@ -326,10 +329,10 @@ class PagedKV:
         """lnskv_sink_decode: every sequence attends its first n_sink tokens and its
         last `window` (0: all of them)."""
         n_seq, stride, out, ws_bytes = self._variant_common(q, tables, kv_len, n_heads, gate, workspace, out)
-        with _on(self.device):
-            check(lib().lnskv_sink_decode(self._c, _ptr(q), _ptr(out), _ptr(gate), _ptr(tables), stride, _ptr(kv_len),
-                                          n_seq, n_heads, max_kv_len, window, n_sink, scale, _ptr(workspace),
-                                          ws_bytes, _stream(self.device)))
+        with _on(self.device) as stream:
+            check(lib().lnskv_sink_decode(self._c, _address(q), out.data_ptr(), _address(gate), tables.data_ptr(), stride, kv_len.data_ptr(),
+                                          n_seq, n_heads, max_kv_len, window, n_sink, scale, _address(workspace),
+                                          ws_bytes, stream))
         return out
 
     def sink_prefill_attention(self, q, chunks, tables, *, n_heads: int, scale: float, window: int, n_sink: int,
@@ -345,10 +348,10 @@ class PagedKV:
         if out is None:
             out = torch.empty((n_tok, n_heads, self.head_dim), dtype=torch.float32, device=self.device)
         _need(out, "out", torch.float32, q.numel(), self.device)
-        with _on(self.device):
-            check(lib().lnskv_sink_prefill_attention(self._c, _ptr(q), _ptr(out), _ptr(chunks), int(chunks.shape[0]),
-                                                     n_tok, _ptr(tables), stride, int(tables.shape[0]), window,
-                                                     n_sink, n_heads, scale, _stream(self.device)))
+        with _on(self.device) as stream:
+            check(lib().lnskv_sink_prefill_attention(self._c, _address(q), out.data_ptr(), chunks.data_ptr(), int(chunks.shape[0]),
+                                                     n_tok, tables.data_ptr(), stride, int(tables.shape[0]), window,
+                                                     n_sink, n_heads, scale, stream))
         return out
 
     def prefix_workspace_size(self, groups: "PrefixGroups", n_seq: int, n_heads: int, max_kv_len: int) -> int:
@@ -363,10 +366,10 @@ class PagedKV:
         """lnskv_prefix_decode: decode in which the sequences of each group read
         their shared leading pages once for all (from the group's first row)."""
         n_seq, stride, out, ws_bytes = self._variant_common(q, tables, kv_len, n_heads, gate, workspace, out)
-        with _on(self.device):
-            check(lib().lnskv_prefix_decode(self._c, _ptr(q), _ptr(out), _ptr(gate), _ptr(tables), stride,
-                                            _ptr(kv_len), groups._p, groups.n, n_seq, n_heads, max_kv_len, scale,
-                                            _ptr(workspace), ws_bytes, _stream(self.device)))
+        with _on(self.device) as stream:
+            check(lib().lnskv_prefix_decode(self._c, _address(q), out.data_ptr(), _address(gate), tables.data_ptr(), stride,
+                                            kv_len.data_ptr(), groups._p, groups.n, n_seq, n_heads, max_kv_len, scale,
+                                            _address(workspace), ws_bytes, stream))
         return out
 
     def attention_paged(self, q, k_in, v_in, block_table, pos: int, n_heads: int, p_start: int = 0,
