@@ -318,7 +318,12 @@ int lnskv_mrope_append(const lnskv_pages* c, const lnskv_rope* rope, const int32
  * and n_sink, same current device) or NULL.  Every page type and shape of
  * lnskv_decode; n_sink in [0, 2^30].
  * lnskv_sink_prefill_attention: lnskv_prefill_attention with this rule (f16 or
- * Q8A pages, head_dim 128 or 256).
+ * Q8A pages, head_dim 128 or 256).  Few query tiles on long windows are split
+ * along the keys, into partial rows in workspace_dev (16-byte aligned,
+ * lnskv_sink_prefill_workspace_size bytes, 0 where nothing is split; a smaller one
+ * is not used and nothing is split; no header to zero) or, where that is NULL, in the
+ * library's decode buffer (calls that use it must not overlap in time; while a
+ * stream is captured it is used only if it is large enough already).
  * ------------------------------------------------------------------------- */
 int lnskv_sink_decode_workspace_size(const lnskv_pages* c, int32_t n_seq, int32_t n_heads,
                                      int32_t max_kv_len, int32_t window, int32_t n_sink, size_t* bytes);
@@ -327,11 +332,14 @@ int lnskv_sink_decode(const lnskv_pages* c, const float* q_dev, float* out_dev, 
                       int32_t n_seq, int32_t n_heads, int32_t max_kv_len, int32_t window,
                       int32_t n_sink, float scale, void* workspace_dev, size_t ws_bytes,
                       lnskv_stream_t stream);
+int lnskv_sink_prefill_workspace_size(const lnskv_pages* c, int32_t n_chunks, int32_t n_tok,
+                                      int32_t bt_stride, int32_t window, int32_t n_sink,
+                                      int32_t n_heads, size_t* bytes);
 int lnskv_sink_prefill_attention(const lnskv_pages* c, const float* q_dev, float* out_dev,
                                  const int32_t* chunks_dev, int32_t n_chunks, int32_t n_tok,
                                  const uint32_t* block_tables_dev, int32_t bt_stride, int32_t n_rows,
                                  int32_t window, int32_t n_sink, int32_t n_heads, float scale,
-                                 lnskv_stream_t stream);
+                                 void* workspace_dev, size_t ws_bytes, lnskv_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Shared prefixes: lnskv_decode for a batch in which runs of sequences begin

@@ -582,7 +582,12 @@ struct PrefillArgs {
   int32_t n_heads;
   uint32_t num_pages;
   float scale_log2;
-  int32_t n_sink;          // launch_prefill_mfma_sink: tokens t < n_sink are attended too
+  // launch_prefill_mfma_sink: tokens t < n_sink are attended too; `splits`
+  // workgroups per tile, with partial rows [n_tok][n_heads][splits] where > 1
+  int32_t n_sink;
+  int32_t splits;
+  float* part_acc;
+  float* part_ml;
 };
 // Queries per tile of the prefill kernel (a workgroup per tile and kv head).
 int prefill_queries_per_tile(int rep, int head_dim);

@@ -1096,10 +1096,27 @@ int lnskv_gated_append_decode(const lnskv_pages* c, const lnskv_rope* rope, cons
 
 namespace lnskv {
 namespace {
+// Workgroups that share a tile's pairs in the prefill with sinks: as many as fill
+// the compute units (a workgroup takes one whole) while each keeps 16 pairs.
+// 812 queries of 4 x 256-wide Q8A kv heads on 2048 + 16 tokens (104 tiles): SPLIT_US
+int sink_prefill_splits(const lnskv_pages* c, int n_chunks, int n_tok, int bt_stride, int window, int n_sink,
+                        int n_heads) {
+  const int qt = prefill_queries_per_tile(n_heads / (int)c->n_kv_heads, (int)c->head_dim);
+  const int64_t tiles = (int64_t)(n_tok + qt - 1) / qt + (n_chunks - 1) / 2;  // chunks' last tiles are half full
+  const int64_t all = (int64_t)bt_stride * kPage;
+  const int64_t tokens = window > 0 ? std::min(all, (int64_t)window + qt + n_sink) : all;
+  const int64_t fill = 256 / std::max<int64_t>(1, tiles * c->n_kv_heads);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({fill, tokens / (16 * 2 * kPage), 16}));
+}
+// The library's decode buffer keeps its header of counts: the rows follow it.
+size_t sink_prefill_bytes(const lnskv_pages* c, int splits, int n_tok, int n_heads) {
+  return kWsHeaderBytes + (size_t)splits * n_tok * n_heads * ((size_t)c->head_dim + 2) * sizeof(float);
+}
 // n_sink < 0: without sinks
 int prefill_entry(const lnskv_pages* c, const float* q, float* out, const int32_t* chunks, int32_t n_chunks,
                   int32_t n_tok, const uint32_t* bt, int32_t bt_stride, int32_t n_rows, const int32_t* p_start,
-                  int32_t window, int32_t n_sink, int32_t n_heads, float scale, lnskv_stream_t stream) {
+                  int32_t window, int32_t n_sink, int32_t n_heads, float scale, void* ws, size_t ws_bytes,
+                  lnskv_stream_t stream) {
   clear_error();
   if (int rc = check_pages(c)) return rc;
   if (!q || !out || !chunks || !bt) return fail(LNSKV_ERR_INVALID, "q, out, chunks and block tables must be non-null");
@@ -1144,7 +1161,26 @@ int prefill_entry(const lnskv_pages* c, const float* q, float* out, const int32_
   const int64_t qt = prefill_queries_per_tile(rep, (int)c->head_dim);
   const int64_t tiles = ((int64_t)n_tok + qt - 1) / qt + n_chunks;
   if (tiles * c->n_kv_heads > INT32_MAX) return fail(LNSKV_ERR_INVALID, "too many query tiles");
-  if (n_sink >= 0) return launch_prefill_mfma_sink(a, rep, (int)c->head_dim, (int)tiles, (hipStream_t)stream);
+  if (n_sink >= 0) {
+    a.splits = sink_prefill_splits(c, n_chunks, n_tok, bt_stride, window, n_sink, n_heads);
+    if (a.splits > 1) {
+      const size_t need = sink_prefill_bytes(c, a.splits, n_tok, n_heads);
+      const bool own = ws == nullptr;
+      if (own && library_buffer(0, need, &ws, (hipStream_t)stream) != LNSKV_OK) {
+        clear_error();
+        ws = nullptr;
+      }
+      if (ws && !aligned16(ws)) return fail(LNSKV_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+      if (ws && (own || ws_bytes >= need)) {
+        a.part_acc = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kWsHeaderBytes);
+        a.part_ml = a.part_acc + (size_t)a.splits * n_tok * n_heads * c->head_dim;
+      } else {
+        a.splits = 1;  // no room for partial rows: one workgroup per tile
+      }
+    }
+    if (tiles * c->n_kv_heads * a.splits > INT32_MAX) return fail(LNSKV_ERR_INVALID, "too many query tiles");
+    return launch_prefill_mfma_sink(a, rep, (int)c->head_dim, (int)tiles, (hipStream_t)stream);
+  }
   return launch_prefill_mfma(a, rep, (int)c->head_dim, (int)tiles, (hipStream_t)stream);
 }
 }  // namespace
@@ -1155,17 +1191,32 @@ int lnskv_prefill_attention(const lnskv_pages* c, const float* q, float* out, co
                             const int32_t* p_start, int32_t window, int32_t n_heads, float scale,
                             lnskv_stream_t stream) {
   return prefill_entry(c, q, out, chunks, n_chunks, n_tok, bt, bt_stride, n_rows, p_start, window, -1, n_heads, scale,
-                       stream);
+                       nullptr, 0, stream);
 }
 
 int lnskv_sink_prefill_attention(const lnskv_pages* c, const float* q, float* out, const int32_t* chunks,
                                  int32_t n_chunks, int32_t n_tok, const uint32_t* bt, int32_t bt_stride,
                                  int32_t n_rows, int32_t window, int32_t n_sink, int32_t n_heads, float scale,
-                                 lnskv_stream_t stream) {
+                                 void* ws, size_t ws_bytes, lnskv_stream_t stream) {
   clear_error();
   if (n_sink < 0 || n_sink > (1 << 30)) return fail(LNSKV_ERR_INVALID, "n_sink %d out of range [0, 2^30]", n_sink);
   return prefill_entry(c, q, out, chunks, n_chunks, n_tok, bt, bt_stride, n_rows, nullptr, window, n_sink, n_heads,
-                       scale, stream);
+                       scale, ws, ws_bytes, stream);
+}
+
+int lnskv_sink_prefill_workspace_size(const lnskv_pages* c, int32_t n_chunks, int32_t n_tok, int32_t bt_stride,
+                                      int32_t window, int32_t n_sink, int32_t n_heads, size_t* bytes) {
+  clear_error();
+  if (!bytes) return fail(LNSKV_ERR_INVALID, "bytes is NULL");
+  *bytes = 0;
+  if (int rc = check_geometry(c)) return rc;
+  const int rep = n_heads / (int)c->n_kv_heads;
+  if (n_chunks <= 0 || n_tok <= 0 || bt_stride <= 0 || window < 0 || n_sink < 0 || n_sink > (1 << 30) || n_heads <= 0 ||
+      n_heads % (int)c->n_kv_heads != 0 || (rep != 1 && rep != 2 && rep != 4 && rep != 8))
+    return fail(LNSKV_ERR_INVALID, "bad shape");
+  const int splits = sink_prefill_splits(c, n_chunks, n_tok, bt_stride, window, n_sink, n_heads);
+  if (splits > 1) *bytes = sink_prefill_bytes(c, splits, n_tok, n_heads);
+  return LNSKV_OK;
 }
 
 int lnskv_split_gated_query(const float* input, float* q_out, float* gate_out, int32_t n_rows, int32_t n_heads,

@@ -479,6 +479,8 @@ __device__ __forceinline__ int pf_tiles(const PrefillArgs& a, int i) {
 // SINK: queries attend the first n_sink tokens besides their window, as two
 // runs of pairs through the same loop: [0, n_sink), then [max(start, n_sink),
 // position]; the limits that the loop holds change where the second begins.
+// Where the tiles do not fill the GPU, a.splits workgroups share a tile's pairs and
+// leave partial rows (numerator, running max, sum) for prefill_merge_kernel.
 template <int REP, bool Q8 = false, int NH = 1, bool SINK = false>
 __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_kernel(PrefillArgs a) {
   using Sh = PfShape<REP, NH>;
@@ -497,6 +499,11 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
   // more chunks are taken in index order.
   const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
   int slot = (int)(blockIdx.x / (unsigned)a.n_kv), c = -1, tile = 0, nt_c = 0;
+  [[maybe_unused]] int split = 0;
+  if constexpr (SINK) {
+    split = slot % a.splits;
+    slot /= a.splits;
+  }
   if (a.n_chunks <= kWave) {
     const int nt = pf_tiles<QT>(a, lane);
     const int4 chl = a.chunks[lane < a.n_chunks ? lane : 0];
@@ -562,7 +569,7 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
   const uint32_t* bt_row = a.bt + (size_t)s * a.bt_stride;
   int pg_first = ta / kPage;
   int npg = ta < tb ? (tb - 1) / kPage - pg_first + 1 : 0;
-  [[maybe_unused]] int sink_pairs = 0, gap = 0;
+  [[maybe_unused]] int sink_pairs = 0, sink_pages = 0, gap = 0;
   [[maybe_unused]] const int tb_w = tb;
   if constexpr (SINK) {
     if (npg > 0) {  // the window's pages, then the sinks' pairs in front of them
@@ -570,20 +577,33 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
       npg = lo < tb ? (tb - 1) / kPage - lo / kPage + 1 : 0;
       sink_pairs = (min(a.n_sink, tb) + 2 * kPage - 1) / (2 * kPage);
       gap = lo / kPage - 2 * sink_pairs;  // table entries left out: may be negative (a page read twice)
-      npg += 2 * sink_pairs;
-      pg_first = sink_pairs > 0 ? 0 : gap;
-      if (sink_pairs > 0) {
-        ta = qlo = 0;
-        tb = min(a.n_sink, tb);
-      }
+      sink_pages = 2 * sink_pairs;
+      npg += sink_pages;
     }
   }
-  const int npairs = (npg + 1) / 2;
-  int base = SINK ? 0 : pg_first;
+  int npairs = (npg + 1) / 2;
+  [[maybe_unused]] int first_pair = 0;
+  if constexpr (SINK) {
+    // this workgroup's pairs: [first_pair, npairs)
+    const int per = (npairs + a.splits - 1) / a.splits;
+    first_pair = min(npairs, split * per);
+    npairs = min(npairs, first_pair + per);
+    if (first_pair < sink_pairs) {
+      pg_first = 0;
+      ta = qlo = 0;
+      tb = min(a.n_sink, tb);
+    } else {
+      pg_first = gap;
+      ta = max(ta, a.n_sink);
+      qlo = max(qlo, a.n_sink);
+      sink_pairs = -1;  // past them already
+    }
+  }
+  int base = SINK ? 2 * first_pair : pg_first;
   uint32_t btv = 0;
   auto load_window = [&]() {
     int e = base + lane;
-    if constexpr (SINK) e = e < 2 * sink_pairs ? e : e + gap;  // base counts the pages of both runs
+    if constexpr (SINK) e = e < sink_pages ? e : e + gap;  // base counts the pages of both runs
     btv = e < a.bt_stride ? bt_row[e] : 0u;
     wait_vmcnt<0>();
   };
@@ -652,7 +672,7 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
   };
 #pragma unroll
   for (int i = 0; i < 2 * kPfBatch; ++i)
-    if (i < npairs) issue(i);
+    if ((SINK ? first_pair + i : i) < npairs) issue(SINK ? first_pair + i : i);
 
   // q -> B operands: per query and head, scale by 2^-E (E from max |q *
   // scale|) so that hi and lo stay in f16 range; scores are scaled back by 2^E
@@ -694,7 +714,7 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
   // kPfBatch pairs per barrier: pairs [i0, i0 + B) are consumed while the
   // next B are in flight and the B after those are issued into the slots of
   // [i0 - B, i0) (every wave consumed those before this barrier).
-  for (int i0 = 0; i0 < npairs; i0 += kPfBatch) {
+  for (int i0 = SINK ? first_pair : 0; i0 < npairs; i0 += kPfBatch) {
     // the pairs issued after this batch, which may stay in flight
     const int later = min(max(npairs - (i0 + kPfBatch), 0), kPfBatch);
     if constexpr (kPfBatch >= 3) {
@@ -726,7 +746,7 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
       const lds_u8* sc = ring + sl * kRingSlot + kPfCodeSlot<NH> + w * kPfScaleWave;  // Q8: this wave's scales
       const bool v0 = (vbits >> (2 * sl)) & 1u, v1 = (vbits >> (2 * sl + 1)) & 1u;
       if constexpr (SINK) {
-        if (i == sink_pairs && sink_pairs > 0) {  // the window begins
+        if (i == sink_pairs) {  // the window begins
           pg_first = gap;
           const int win = a.window > 0 ? a.window : INT32_MAX;
           ta = max(pos0 - win + 1, a.n_sink);
@@ -755,6 +775,34 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
   }
   if (!active) return;
 
+  if constexpr (SINK) {  // partial rows [token][head][split], or with one split the output rows
+    // the wave's queries and heads again, not held through the loop (two registers spilled)
+    int we = (int)(threadIdx.x / kWave);
+    asm volatile("" : "+v"(we));
+    const int te = QT * tile + 16 * (we / WPQ), qn_e = min(16, ch.z - te), he = kvh * REP + (we % WPQ) * HW;
+    const bool whole = a.splits == 1;
+    float* dst = whole ? a.out : a.part_acc;
+#pragma unroll
+    for (int hh = 0; hh < HW; ++hh) {
+      const float lt = sum_xor16(sum_xor32(l[hh]));
+#pragma unroll
+      for (int ii = 0; ii < 4; ++ii) {
+        const float L = __shfl(lt, 20 * g + ii, kWave);  // query 4g + ii
+        const float M = __shfl(m[hh], 20 * g + ii, kWave);
+        if (4 * g + ii < qn_e) {
+          const size_t r = ((size_t)(ch.w + te + 4 * g + ii) * a.n_heads + he + hh) * a.splits + split;
+          const float f = (Q8 ? vnorm : 1.0f) * (whole ? (L > 0.0f ? 1.0f / L : 0.0f) : 1.0f);
+          if (!whole && n == 0) {
+            a.part_ml[2 * r] = M;
+            a.part_ml[2 * r + 1] = L;
+          }
+#pragma unroll
+          for (int nb = 0; nb < 8 * NH; ++nb) dst[r * (NH * kD) + 16 * nb + n] = acc[hh][nb][ii] * f;
+        }
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int hh = 0; hh < HW; ++hh) {
     // l over the 32 tokens of each pair: sum the four lanes of query n
@@ -773,9 +821,36 @@ __global__ __launch_bounds__((kWave * PfShape<REP, NH>::NW)) void prefill_mfma_k
   }
 }
 
+// Joins the partial rows of a split launch: wave per (token, head); tokens in no
+// chunk are left alone.
+template <int D>
+__global__ __launch_bounds__(kBlock) void prefill_merge_kernel(PrefillArgs a) {
+  constexpr int C = D / kWave;
+  const int64_t i = (int64_t)blockIdx.x * kWavesPerBlock + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  if (i >= (int64_t)a.n_tok * a.n_heads) return;  // wave-uniform
+  const int t = (int)(i / a.n_heads);
+  bool covered = false;
+  for (int c0 = 0; c0 < a.n_chunks && !covered; c0 += kWave) {
+    bool hit = false;
+    if (pf_tiles<1>(a, c0 + lane) > 0) {
+      const int4 ch = a.chunks[c0 + lane];
+      hit = t >= ch.w && t - ch.w < ch.z;
+    }
+    covered = __builtin_amdgcn_ballot_w64(hit) != 0;
+  }
+  if (!covered) return;
+  float M, Ls, A[C];
+  const size_t r0 = (size_t)i * a.splits;
+  merge_wave<D, 1, 4>(reinterpret_cast<const float2*>(a.part_ml), a.part_acc, 0, a.splits,
+                      [=](int j) { return r0 + (size_t)j; }, M, Ls, A);
+#pragma unroll
+  for (int c = 0; c < C; ++c) a.out[(size_t)i * D + c * kWave + lane] = Ls > 0.0f ? A[c] / Ls : 0.0f;
+}
+
 template <int REP, int NH, bool SINK>
 void launch_prefill_rep(const PrefillArgs& a, int n_tiles, hipStream_t st) {
-  const unsigned blocks = (unsigned)n_tiles * (unsigned)a.n_kv;
+  const unsigned blocks = (unsigned)n_tiles * (unsigned)a.n_kv * (SINK ? (unsigned)a.splits : 1u);
   if (a.k_scales)
     prefill_mfma_kernel<REP, true, NH, SINK><<<blocks, kWave * PfShape<REP, NH>::NW, 0, st>>>(a);
   else

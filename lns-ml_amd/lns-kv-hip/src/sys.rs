@@ -285,6 +285,16 @@ extern "C" {
         ws_bytes: usize,
         stream: HipStream,
     ) -> c_int;
+    pub fn lnskv_sink_prefill_workspace_size(
+        c: *const LnskvPages,
+        n_chunks: i32,
+        n_tok: i32,
+        bt_stride: i32,
+        window: i32,
+        n_sink: i32,
+        n_heads: i32,
+        bytes: *mut usize,
+    ) -> c_int;
     pub fn lnskv_sink_prefill_attention(
         c: *const LnskvPages,
         q_dev: *const f32,
@@ -299,6 +309,8 @@ extern "C" {
         n_sink: i32,
         n_heads: i32,
         scale: f32,
+        workspace_dev: *mut c_void,
+        ws_bytes: usize,
         stream: HipStream,
     ) -> c_int;
     pub fn lnskv_prefix_decode_workspace_size(

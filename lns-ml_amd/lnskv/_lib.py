@@ -137,7 +137,8 @@ SIGNATURES = {
     "lnskv_sink_decode": (
         C.c_int, [_P, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
     "lnskv_sink_prefill_attention": (
-        C.c_int, [_P, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
+        C.c_int, [_P, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
+    "lnskv_sink_prefill_workspace_size": (C.c_int, [_P, _i32, _i32, _i32, _i32, _i32, _i32, C.POINTER(_sz)]),
     "lnskv_prefix_decode_workspace_size": (C.c_int, [_P, _vp, _i32, _i32, _i32, _i32, C.POINTER(_sz)]),
     "lnskv_prefix_decode": (
         C.c_int, [_P, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),

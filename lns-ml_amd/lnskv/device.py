@@ -335,8 +335,15 @@ class PagedKV:
                                           ws_bytes, stream))
         return out
 
+    def sink_prefill_workspace_size(self, n_chunks: int, n_tok: int, stride: int, window: int, n_sink: int,
+                                    n_heads: int) -> int:
+        out = C.c_size_t()
+        check(lib().lnskv_sink_prefill_workspace_size(self._c, n_chunks, n_tok, stride, window, n_sink, n_heads,
+                                                      C.byref(out)))
+        return out.value
+
     def sink_prefill_attention(self, q, chunks, tables, *, n_heads: int, scale: float, window: int, n_sink: int,
-                               out=None) -> torch.Tensor:
+                               workspace=None, out=None) -> torch.Tensor:
         """lnskv_sink_prefill_attention: prefill_attention whose queries attend the
         first n_sink tokens besides their own window."""
         n_tok = q.numel() // (n_heads * self.head_dim)
@@ -348,10 +355,14 @@ class PagedKV:
         if out is None:
             out = torch.empty((n_tok, n_heads, self.head_dim), dtype=torch.float32, device=self.device)
         _need(out, "out", torch.float32, q.numel(), self.device)
+        ws_bytes = 0
+        if workspace is not None:
+            _need(workspace, "workspace", workspace.dtype, workspace.numel(), self.device)
+            ws_bytes = workspace.numel() * workspace.element_size()
         with _on(self.device) as stream:
             check(lib().lnskv_sink_prefill_attention(self._c, _address(q), out.data_ptr(), chunks.data_ptr(), int(chunks.shape[0]),
                                                      n_tok, tables.data_ptr(), stride, int(tables.shape[0]), window,
-                                                     n_sink, n_heads, scale, stream))
+                                                     n_sink, n_heads, scale, _address(workspace), ws_bytes, stream))
         return out
 
     def prefix_workspace_size(self, groups: "PrefixGroups", n_seq: int, n_heads: int, max_kv_len: int) -> int:

@@ -238,3 +238,35 @@ def test_decode_on_another_stream_and_wrong_inputs():
         pk.sink_decode(q.transpose(1, 2), t, kl, **call)
     with pytest.raises(TypeError):
         pk.sink_decode(q.half(), t, kl, **call)
+
+
+@pytest.mark.parametrize("dtype,d,rep", [(DTYPE_F16, 128, 4), (DTYPE_Q8A, 256, 4), (DTYPE_F16, 256, 1), (DTYPE_Q8A, 128, 8)])
+def test_prefill_split_along_the_keys(dtype, d, rep):
+    """Few queries on a long window: with a workspace, the library's buffer and a
+    workspace too small to split; rows of no chunk keep what they hold."""
+    say("sink prefill split", dtype, d, rep)
+    rng = np.random.default_rng(5)
+    chunks, window, sink = [(5000, 37), (2990, 20)], 2500, 600
+    lens = [a + b for a, b in chunks]
+    seen = [[t for t in range(L) if t < sink or t > a - window] for (a, _), L in zip(chunks, lens)]
+    tables, n = A.make_tables(lens, [sorted({t // 16 for t in x}) for x in seen], rng)
+    pk = PagedKV(n, 1, d, dtype, DEV)
+    A.fill(pk, 5)
+    A.poison(pk, np.concatenate([A.slots_of(tables[s], x, n) for s, x in enumerate(seen)]))
+    n_tok, scale = 64, 1.0 / np.sqrt(d)
+    q = (2 * rng.standard_normal((n_tok, rep, d))).astype(np.float32)
+    vals, ref = A.values(pk), np.full((n_tok, rep, d), 7.0)
+    desc = np.array([[0, 5000, 37, 0], [1, 2990, 20, 40]], np.int32)
+    for s, a, b, at in desc:
+        for i in range(b):
+            tok = [t for t in range(a + i + 1) if t < sink or t > a + i - window]
+            ref[at + i] = A.row(vals, q[at + i], A.slots_of(tables[s], tok, n), scale)
+    size = pk.sink_prefill_workspace_size(2, n_tok, tables.shape[1], window, sink, rep)
+    assert size > 0
+    for ws in (torch.full((size,), 0xFF, dtype=torch.uint8, device=DEV), None, torch.zeros(64, dtype=torch.uint8, device=DEV)):
+        out = torch.full((n_tok, rep, d), 7.0, device=DEV)
+        pk.sink_prefill_attention(dev_f32(q, DEV), dev_i32(desc, DEV), dev_i32(tables, DEV), n_heads=rep, scale=scale,
+                                  window=window, n_sink=sink, workspace=ws, out=out)
+        torch.cuda.synchronize()
+        assert A.worst(out, ref) < A.TOL
+        assert (out[37:40] == 7.0).all() and (out[60:] == 7.0).all()

@@ -113,7 +113,7 @@ def test_prefix_decode_refuses(kw, rc, text):
 def test_sink_prefill_refuses():
     def call(c, window=16, n_sink=4, n_heads=8, chunks=P):
         return status("lnskv_sink_prefill_attention", C.byref(c), P, P, chunks, 1, 4, P, 4, 1, window, n_sink, n_heads, 0.1,
-                      None)
+                      None, 0, None)
     f16 = pages(_lib.DTYPE_F16, 128)
     for c, kw, rc, text in [(pages(_lib.DTYPE_F16, 64), {}, UNS, "head_dim"), (pages(d=128), {}, UNS, "f16 and Q8A"),
                             (f16, dict(window=-1), INV, "window"), (f16, dict(n_sink=-1), INV, "n_sink"),
