@@ -1,18 +1,18 @@
 // Host side shared by the decode variants (kSink, kPrefix): the checks of a
-// call, its arguments and workspace, and the generic kernel's launches.
+// call, its arguments and workspace, and the tile kernel's launches.
 #pragma once
 
 #include <cmath>
 
 #include <algorithm>
 
-#include "lnskv_decode_valu.h"
+#include "lnskv_decode_tile.h"
 
 namespace lnskv {
 namespace {
 
 // How a call runs.  On f16 and Q8A pages with head_dim 128 or 256 (var_mfma) each
-// variant has schedules of its own; on other pages the generic kernel runs in
+// variant has schedules of its own; on other pages the tile kernel runs in
 // partitions of `split` tokens.
 struct VarPlan {
   int wg = 0;        // kSink: the workgroup schedule
@@ -22,18 +22,19 @@ struct VarPlan {
   size_t ws_bytes = 0;
 };
 
-constexpr int kOnePartition = 192;
+constexpr int kOnePartition = 256;  // tokens
+constexpr int kLeastPartition = 128;
 
 inline bool var_mfma(const lnskv_pages* c) {
   return c->dtype != LNSKV_DTYPE_F32 && (c->head_dim == 128 || c->head_dim == 256);
 }
 
-// The generic kernel's partitions for sequences of at most `pages` pages: one
+// The tile kernel's partitions for sequences of at most `pages` pages: one
 // where those are few (a block's four waves share it and no merge is launched).
-inline int plan_generic(const lnskv_pages* c, int n_seq, int n_heads, int64_t pages, VarPlan* p) {
+inline int plan_tiles(const lnskv_pages* c, int n_seq, int n_heads, int64_t pages, VarPlan* p) {
   const int64_t tokens = std::max<int64_t>(pages, 1) * kPage;
   p->split = tokens <= kOnePartition ? (int)tokens
-                                     : choose_split(n_seq, (int)c->n_kv_heads, (int)std::min<int64_t>(tokens, INT32_MAX / 2));
+                                     : std::max(kLeastPartition, choose_split(n_seq, (int)c->n_kv_heads, (int)std::min<int64_t>(tokens, INT32_MAX / 2)));
   const int64_t parts = (tokens + p->split - 1) / p->split;
   if (parts > 65535)
     return fail(LNSKV_ERR_INVALID, "%lld tokens a sequence need more than 65535 partitions", (long long)tokens);
@@ -43,19 +44,19 @@ inline int plan_generic(const lnskv_pages* c, int n_seq, int n_heads, int64_t pa
 }
 
 template <int VAR, int DT, int D, int REP>
-void launch_var_valu(const DecodeArgs& a, const VarArgs<VAR>& x, int n_seq, hipStream_t st) {
+void launch_tile(const DecodeArgs& a, const VarArgs<VAR>& x, int n_seq, hipStream_t st) {
   const dim3 grid((unsigned)a.n_kv, (unsigned)a.max_parts, (unsigned)n_seq);
-  decode_valu_kernel<DT, D, REP, false, VAR><<<grid, kBlock, 0, st>>>(a, x);
+  decode_tile_kernel<DT, D, REP, VAR><<<grid, kBlock, 0, st>>>(a, x);
   launch_combine<REP, D, false, VAR>(a, n_seq, st, x);
 }
 
 template <int VAR, int DT, int D>
-int launch_var_valu_rep(const DecodeArgs& a, const VarArgs<VAR>& x, int rep, int n_seq, hipStream_t st) {
+int launch_tile_rep(const DecodeArgs& a, const VarArgs<VAR>& x, int rep, int n_seq, hipStream_t st) {
   switch (rep) {
-    case 1: launch_var_valu<VAR, DT, D, 1>(a, x, n_seq, st); break;
-    case 2: launch_var_valu<VAR, DT, D, 2>(a, x, n_seq, st); break;
-    case 4: launch_var_valu<VAR, DT, D, 4>(a, x, n_seq, st); break;
-    default: launch_var_valu<VAR, DT, D, 8>(a, x, n_seq, st); break;
+    case 1: launch_tile<VAR, DT, D, 1>(a, x, n_seq, st); break;
+    case 2: launch_tile<VAR, DT, D, 2>(a, x, n_seq, st); break;
+    case 4: launch_tile<VAR, DT, D, 4>(a, x, n_seq, st); break;
+    default: launch_tile<VAR, DT, D, 8>(a, x, n_seq, st); break;
   }
   return hip_check("decode kernel launch");
 }
@@ -105,9 +106,9 @@ inline DecodeArgs var_args(const lnskv_pages* c, const float* q, float* out, con
   return a;
 }
 
-// Launches the generic kernel; ws: plan.ws_bytes of workspace.
+// Launches the tile kernel; ws: plan.ws_bytes of workspace.
 template <int VAR>
-int launch_generic(const lnskv_pages* c, DecodeArgs a, const VarPlan& plan, int n_seq, void* ws, const VarArgs<VAR>& x,
+int launch_tiles(const lnskv_pages* c, DecodeArgs a, const VarPlan& plan, int n_seq, void* ws, const VarArgs<VAR>& x,
                    hipStream_t st) {
   const int d = (int)c->head_dim, rep = a.n_heads / a.n_kv;
   if (plan.ws_bytes > 0) {
@@ -116,13 +117,13 @@ int launch_generic(const lnskv_pages* c, DecodeArgs a, const VarPlan& plan, int 
   }
   if (c->dtype == LNSKV_DTYPE_F32) {
     switch (d) {
-      case 64: return launch_var_valu_rep<VAR, LNSKV_DTYPE_F32, 64>(a, x, rep, n_seq, st);
-      case 128: return launch_var_valu_rep<VAR, LNSKV_DTYPE_F32, 128>(a, x, rep, n_seq, st);
-      default: return launch_var_valu_rep<VAR, LNSKV_DTYPE_F32, 256>(a, x, rep, n_seq, st);
+      case 64: return launch_tile_rep<VAR, LNSKV_DTYPE_F32, 64>(a, x, rep, n_seq, st);
+      case 128: return launch_tile_rep<VAR, LNSKV_DTYPE_F32, 128>(a, x, rep, n_seq, st);
+      default: return launch_tile_rep<VAR, LNSKV_DTYPE_F32, 256>(a, x, rep, n_seq, st);
     }
   }
-  if (c->dtype == LNSKV_DTYPE_Q8A) return launch_var_valu_rep<VAR, LNSKV_DTYPE_Q8A, 64>(a, x, rep, n_seq, st);
-  return launch_var_valu_rep<VAR, LNSKV_DTYPE_F16, 64>(a, x, rep, n_seq, st);
+  if (c->dtype == LNSKV_DTYPE_Q8A) return launch_tile_rep<VAR, LNSKV_DTYPE_Q8A, 64>(a, x, rep, n_seq, st);
+  return launch_tile_rep<VAR, LNSKV_DTYPE_F16, 64>(a, x, rep, n_seq, st);
 }
 
 // A call's workspace: the caller's, checked, or the library's decode buffer.

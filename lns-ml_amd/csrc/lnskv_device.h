@@ -416,11 +416,27 @@ __device__ __forceinline__ void finish_block(const DecodeArgs& a, EpilogueLds<RE
         const VarArgs<kPrefix>& px = only(x...);
         const PrefixRows pr = prefix_rows(px, s, a.n_heads);
         const size_t r0 = pr.base + (size_t)(h0 + h) * pr.splits;
-        for (int j = 0; j < pr.splits; ++j) {
-          const float ms = px.part_ml[2 * (r0 + j)], ls = px.part_ml[2 * (r0 + j) + 1], Mn = fmaxf(M, ms);
-          const float wa = fast_exp2(M - Mn), wb = fast_exp2(ms - Mn);
-          A = A * wa + px.part_acc[(r0 + j) * D + i] * wb;
-          Ls = Ls * wa + ls * wb;
+        for (int j0 = 0; j0 < pr.splits; j0 += 16) {  // sixteen rows' loads in flight
+          float2 pm[16];
+          float pa[16];
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            const bool in = j0 + u < pr.splits;
+            pm[u] = in ? reinterpret_cast<const float2*>(px.part_ml)[r0 + j0 + u] : make_float2(kMInit, 0.0f);
+            pa[u] = in ? px.part_acc[(r0 + j0 + u) * D + i] : 0.0f;
+          }
+          float Mn = M;
+#pragma unroll
+          for (int u = 0; u < 16; ++u) Mn = fmaxf(Mn, pm[u].x);
+          const float wa = fast_exp2(M - Mn);
+          A *= wa;
+          Ls *= wa;
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            const float wb = fast_exp2(pm[u].x - Mn);
+            A = fmaf(wb, pa[u], A);
+            Ls = fmaf(wb, pm[u].y, Ls);
+          }
           M = Mn;
         }
       }

@@ -9,7 +9,7 @@
 //    pages, kv head).  A row is one query head of one sequence; all rows of a
 //    tile multiply the same K and V.  Each item leaves a partial row (A, m, l)
 //    per query row.
-// 2. own kernel (f16 and Q8A pages, 128- and 256-wide heads; the generic decode
+// 2. own kernel (f16 and Q8A pages, 128- and 256-wide heads; the tile kernel's
 //    kernel elsewhere): work item = (sequence, kv head, share of its own pages);
 //    a sequence with one share merges the prefix's rows and writes its output.
 // 3. join kernel, where sequences may have several shares: their rows and the
@@ -21,10 +21,16 @@
 namespace lnskv {
 namespace {
 
-constexpr int kRowsTile = 64;   // query rows per tile of the f32 kernel: four waves of 16
-constexpr int kSplitPages = 8;     // fewest pages of a split, matrix-core kernel
-constexpr int kSplitPagesF32 = 2;  // f32 kernel
-constexpr int kSharePages = 64;    // most pages of a share of a sequence's own
+// Fewest pages of a split.  Us with 2 | 4 | 8, shared tokens x rows x kv heads: 547 x 164
+// x 8 22.0 | 21.5 | 23.8, 193 x 12 x 4 (256-wide) 26.1 | 27.5 | 31.5, 63 x 16 x 8 12.5 |
+// 13.4 | 13.4; tile kernel 503 x 8 x 8 21.7 | 24.0 | 29.0, 505 x 10 x 8 10.6 | 12.6 | 16.9.
+constexpr int kSplitPages = 2;
+// Splits of 128-row tiles from which tiles of 256 rows read each operand from LDS for
+// twice the products.  Us, 128 | 256 rows, 512 rows x 8 kv heads, f16 pages: 4000 tokens
+// (splits of 32 pages) 42.9 | 45.3, 8000 66.2 | 62.6, 16000 109 | 100; Q8A 51.3 | 50.8,
+// 78.2 | 70.9, 125 | 111.
+constexpr int kWidePages = 48;
+constexpr int kSharePages = 64;  // most pages of a share of a sequence's own
 constexpr int kShareMin = 8;
 
 struct PrefixArgs {
@@ -95,135 +101,50 @@ __device__ __forceinline__ int row_tokens(const PrefixArgs& a, int s, int pages)
 }
 
 // ---------------------------------------------------------------------------
-// f32 pages, and 64-wide heads on every page type, in f32: both products as v_mfma_f32_16x16x4_f32
-// over a page of K and V held in LDS as f32 (Q8A: code x scale).  Wave w holds
-// rows 16w .. 16w + 15 of the tile.  Lane (g, n) = (lane / 16, lane % 16):
-//  S^T[16 tok][16 row] = K . Q^T, product (jj, e) over dims 16 jj + 4 g' + e
-//  (g' = 0..3 the contraction index), so that both operands of four products
-//  are one 16-byte read; lane (g, n) gets tokens 4g + ii of row n.
-//  O[16 row][D] += P . V, product ii over tokens 4 g' + ii: its A operand is the
-//  lane's own weight ii; lane (g, n) accumulates O[row 4g + i][16 nb + n].
-// LDS rows are D + 4 floats: four rows apart fall 16 banks apart.
+// f32 pages, and 64-wide heads on every page type, in f32 (lnskv_decode_tile.h): a
+// wave per item of 16 rows and one split.  The waves of a block take the tiles of
+// one split, or consecutive splits of few rows, and share nothing but the cache.
 template <int DT, int D>
-__global__ __launch_bounds__(kBlock) void prefix_f32_kernel(PrefixArgs a) {
-  constexpr int ES = Storage<DT>::kBytes;
-  constexpr int kStride = D + 4;
-  constexpr int kElems = D / 16;              // elements of a row per thread
-  constexpr int kWords = kElems * ES / 4;     // and their 32-bit words (1 to 16)
-  __shared__ __attribute__((aligned(16))) float ks_[kPage * kStride];
-  __shared__ __attribute__((aligned(16))) float vs_[kPage * kStride];
-  __shared__ int most_[kWavesPerBlock];
+__global__ __launch_bounds__(kBlock) void prefix_tile_kernel(PrefixArgs a) {
   const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
-  const PrefixItem it = prefix_item(a, (int)(blockIdx.x / (unsigned)a.n_kv), kRowsTile);
-  if (it.group < 0) return;  // block-uniform
+  const int wi = (int)(threadIdx.x / kWave), lane = (int)(threadIdx.x % kWave), g = lane >> 4, n = lane & 15;
+  const PrefixItem it = prefix_item(
+      a, __builtin_amdgcn_readfirstlane((int)(blockIdx.x / (unsigned)a.n_kv) * kWavesPerBlock + wi), 16);
+  if (it.group < 0) return;  // wave-uniform; the waves share nothing
   const PrefixGroup gr = a.g[it.group];
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane >> 4, n = lane & 15;
-  const int rows = (gr.end - gr.first) * a.rep;
-  const int r0 = it.tile * kRowsTile + 16 * w;  // this wave's first row
-  const int pg0 = it.split * a.split_pages, pg_end = min(gr.pages, pg0 + a.split_pages);
-
+  const int rows = (gr.end - gr.first) * a.rep, r0 = 16 * it.tile;
   const int rn = min(r0 + n, rows - 1);  // past the last row: that row again, never written
   const int sn = gr.first + rn / a.rep, hn = kvh * a.rep + rn % a.rep;
   const int limit = row_tokens(a, sn, gr.pages);
-  // tokens past every row's length are masked in the whole tile: their V is
-  // zeroed, since 0 * NaN of a stale slot would reach the sums
-  int most = limit;
+  int most = limit, least = limit;
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o, kWave));
-  if (lane == 0) most_[w] = most;
-  __syncthreads();
-  most = max(max(most_[0], most_[1]), max(most_[2], most_[3]));
-  const int pg1 = min(pg_end, (most + kPage - 1) / kPage);
-  float4v q[D / 16];
-  {
-    const float4v* src = reinterpret_cast<const float4v*>(a.q + ((size_t)sn * a.n_heads + hn) * D) + g;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) q[j] = src[4 * j] * a.scale_log2;
+  for (int o = 1; o < 16; o <<= 1) {
+    most = max(most, __shfl_xor(most, o, kWave));
+    least = min(least, __shfl_xor(least, o, kWave));
   }
-  float4v acc[D / 16];
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j) acc[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kMInit, l = 0.0f;
-
-  // this thread's elements of a page: kElems of token threadIdx.x / 16
-  const int tt = threadIdx.x >> 4, tc = (threadIdx.x & 15) * kElems;
-  uint32_t kw[kWords], vw[kWords];
-  float ksc = 1.0f, vsc = 1.0f;
-  bool ok = false;
+  most = __builtin_amdgcn_readfirstlane(most);
+  least = __builtin_amdgcn_readfirstlane(least);
+  const int pg0 = it.split * a.split_pages;
+  const int pg1 = min(min(gr.pages, pg0 + a.split_pages), (most + kPage - 1) / kPage);
   const uint32_t* bt_row = a.bt + (size_t)gr.first * a.bt_stride;
-  auto load = [&](int pg) {
-    const uint32_t ph = pg < a.bt_stride ? bt_row[pg] : 0xFFFFFFFFu;
-    ok = ph < a.num_pages;
-    const size_t slot = (size_t)(ok ? ph : 0u) * kPage + tt;  // a missing page reads page 0, masked
-    const size_t off = ((slot * a.n_kv + kvh) * D + tc) * ES;
-    const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.k_pages + off);
-    const uint32_t* vp = reinterpret_cast<const uint32_t*>(a.v_pages + off);
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      kw[i] = kp[i];
-      vw[i] = vp[i];
-    }
-    if constexpr (DT == LNSKV_DTYPE_Q8A) {
-      ksc = a.k_scales[slot * a.n_kv + kvh];
-      vsc = a.v_scales[slot * a.n_kv + kvh];
-    }
-  };
-  auto value = [](const uint32_t* word, int e, float sc) -> float {
-    const uint32_t x = word[e * ES / 4];
-    if constexpr (DT == LNSKV_DTYPE_F32) return __builtin_bit_cast(float, x);
-    else if constexpr (DT == LNSKV_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(x >> (16 * (e & 1))));
-    else return (float)(int8_t)(x >> (8 * (e & 3))) * sc;
-  };
-  if (pg0 < pg1) load(pg0);
-  for (int pg = pg0; pg < pg1; ++pg) {
-    const bool valid = ok;
-    __syncthreads();  // every wave is done with the page before
-#pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-      ks_[tt * kStride + tc + e] = value(kw, e, ksc);
-      vs_[tt * kStride + tc + e] = valid && pg * kPage + tt < most ? value(vw, e, vsc) : 0.0f;
-    }
-    __syncthreads();
-    if (pg + 1 < pg1) load(pg + 1);
-    float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      const float4v k = *reinterpret_cast<const float4v*>(ks_ + n * kStride + 16 * j + 4 * g);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[j][e], s, 0, 0, 0);
-    }
-    const int tok0 = pg * kPage;
-#pragma unroll
-    for (int ii = 0; ii < 4; ++ii)
-      if (!(valid && tok0 + 4 * g + ii < limit)) s[ii] = -INFINITY;
-    float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    mx = max_xor16(max_xor32(mx));  // over the page's tokens, row n
-    if (__builtin_amdgcn_ballot_w64(mx > m)) {  // wave-uniform
-      const float mn = fmaxf(m, mx), alpha = fast_exp2(m - mn);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float ar = __shfl(alpha, 20 * g + i, kWave);  // row 4g + i
-#pragma unroll
-        for (int nb = 0; nb < D / 16; ++nb) acc[nb][i] *= ar;
-      }
-    }
-    float p[4];
-#pragma unroll
-    for (int ii = 0; ii < 4; ++ii) p[ii] = fast_exp2(s[ii] - m);
-    l += (p[0] + p[1]) + (p[2] + p[3]);
-#pragma unroll
-    for (int ii = 0; ii < 4; ++ii)
-#pragma unroll
-      for (int nb = 0; nb < D / 16; ++nb)
-        acc[nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[ii], vs_[(4 * g + ii) * kStride + 16 * nb + n], acc[nb], 0, 0, 0);
+  TileState<DT, D> st;
+  tile_init<DT, D>(st, a.q + ((size_t)sn * a.n_heads + hn) * D, a.scale_log2, g);
+  for (int p = pg0; p < pg1; p += kWave) {  // 64 table entries at a time
+    const uint32_t btv = p + lane < a.bt_stride ? bt_row[p + lane] : 0xFFFFFFFFu;
+    tile_pages<DT, D>(
+        a, kvh, g, n, 0, 1, min(pg1 - p, kWave), [&](int i) { return __builtin_amdgcn_readlane(btv, i); },
+        [&](int i, bool valid, TilePage<DT, D>& pg) {
+          const int tok0 = (p + i) * kPage;
+          tile_consume<DT, D>(
+              st, pg, valid && tok0 + kPage <= least, g, [&](int t) { return valid && tok0 + t < limit; },
+              [&](int t) { return valid && tok0 + t < most; });
+        });
   }
-  l = sum_xor16(sum_xor32(l));
+  st.l = sum_xor16(sum_xor32(st.l));
   if (lane < 16 && r0 + n < rows) {
     const RowOut o = row_out<D>(a, it, sn, hn);
-    o.ml[0] = m;
-    o.ml[1] = l;
+    o.ml[0] = st.m;
+    o.ml[1] = st.l;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -231,7 +152,9 @@ __global__ __launch_bounds__(kBlock) void prefix_f32_kernel(PrefixArgs a) {
     if (r < rows) {
       const RowOut o = row_out<D>(a, it, gr.first + r / a.rep, kvh * a.rep + r % a.rep);
 #pragma unroll
-      for (int nb = 0; nb < D / 16; ++nb) o.acc[16 * nb + n] = acc[nb][i];
+      for (int c = 0; c < D / 64; ++c)
+        *reinterpret_cast<float4v*>(o.acc + 64 * c + 4 * n) =
+            float4v{st.acc[4 * c][i], st.acc[4 * c + 1][i], st.acc[4 * c + 2][i], st.acc[4 * c + 3][i]};
     }
   }
 }
@@ -602,24 +525,20 @@ void launch_prefix_mfma(const PrefixArgs& a, int d, int tile_rows, unsigned bloc
 }
 
 template <int DT>
-void launch_prefix_f32(const PrefixArgs& a, int d, unsigned blocks, hipStream_t st) {
-  switch (d) {
-    case 64: prefix_f32_kernel<DT, 64><<<blocks, kBlock, 0, st>>>(a); return;
-    default: break;
-  }
+void launch_prefix_tile(const PrefixArgs& a, int d, int64_t items, hipStream_t st) {
+  const unsigned blocks = (unsigned)((items + kWavesPerBlock - 1) / kWavesPerBlock * a.n_kv);
+  if (d == 64) prefix_tile_kernel<DT, 64><<<blocks, kBlock, 0, st>>>(a);
   if constexpr (DT == LNSKV_DTYPE_F32) {
-    if (d == 128)
-      prefix_f32_kernel<DT, 128><<<blocks, kBlock, 0, st>>>(a);
-    else
-      prefix_f32_kernel<DT, 256><<<blocks, kBlock, 0, st>>>(a);
+    if (d == 128) prefix_tile_kernel<DT, 128><<<blocks, kBlock, 0, st>>>(a);
+    if (d == 256) prefix_tile_kernel<DT, 256><<<blocks, kBlock, 0, st>>>(a);
   }
 }
 
 // ---------------------------------------------------------------------------
 // The host's view of a call.
 struct PrefixPlan {
-  VarPlan own;            // the generic kernel over the sequences' own pages
-  int shares = 0;         // own kernel: shares of a sequence at most (0: the generic kernel)
+  VarPlan own;            // the tile kernel over the sequences' own pages
+  int shares = 0;         // own kernel: shares of a sequence at most (0: the tile kernel)
   int share_pages = 0;
   int split_pages = 1;
   int tile_rows = 0;      // query rows of a work item
@@ -636,13 +555,8 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
     return fail(LNSKV_ERR_INVALID, "n_groups %d out of range [0, %d]", n_groups, LNSKV_PREFIX_MAX_GROUPS);
   if (n_groups > 0 && !groups) return fail(LNSKV_ERR_INVALID, "groups must be non-null");
   const int rep = n_heads / (int)c->n_kv_heads, d = (int)c->head_dim;
-  // the matrix-core kernel takes two heads of a sequence per column where some
-  // group has more than 128 rows
-  int most_rows = 0;
-  for (int i = 0; i < n_groups; ++i) most_rows = std::max(most_rows, std::min(groups[3 * i + 1], n_seq) * rep);
-  p->tile_rows = !var_mfma(c) ? kRowsTile : (d == 128 && rep > 1 && most_rows > 128 ? 256 : 128);
   const int64_t all = (int64_t)max_kv_len / kPage + 1;
-  int64_t own_pages = 0, most = 0, tiles = 0, max_shared = 0;  // summed over sequences; of one sequence
+  int64_t own_pages = 0, most = 0, tiles = 0, wide = 0, max_shared = 0;  // summed over sequences; of one sequence
   int at = 0;
   for (int i = 0; i < n_groups; ++i) {
     const int first = groups[3 * i], n = groups[3 * i + 1], tok = groups[3 * i + 2];
@@ -658,7 +572,8 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
     most = std::max(most, std::max<int64_t>(all - shared, 1));
     if (shared == 0) continue;
     p->g[p->n_groups++] = PrefixGroup{first, at, (int32_t)shared};
-    tiles += ceil_div(n * rep, p->tile_rows);
+    tiles += ceil_div(n * rep, var_mfma(c) ? 128 : 16);
+    wide += ceil_div(n * rep, 256);
     max_shared = std::max(max_shared, shared);
   }
   if (at < n_seq) most = all;
@@ -667,7 +582,7 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   if (var_mfma(c)) {
     // shares of at most kSharePages pages, fewer where that leaves compute units idle
     const int64_t units = own_pages * c->n_kv_heads;
-    p->share_pages = n_seq * (int64_t)c->n_kv_heads >= 256
+    p->share_pages = n_seq * (int64_t)c->n_kv_heads >= 256 || most <= 32
                          ? kSharePages
                          : (int)std::min<int64_t>(kSharePages, std::max<int64_t>(kShareMin, (units + 511) / 512));
     p->shares = (int)std::max<int64_t>(1, (most + p->share_pages - 1) / p->share_pages);
@@ -676,14 +591,22 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
     p->own_at = kWsHeaderBytes;
     p->ws_bytes = p->shares > 1 ? kWsHeaderBytes + (size_t)p->shares * n_seq * n_heads * row : 0;
   } else {
-    if (int rc = plan_generic(c, n_seq, n_heads, most, &p->own)) return rc;
+    if (int rc = plan_tiles(c, n_seq, n_heads, most, &p->own)) return rc;
     p->ws_bytes = p->own.ws_bytes;
   }
   if (p->n_groups == 0) return LNSKV_OK;
-  // splits of equal pages, about one matrix-core item or two of the f32 kernel's per
-  // compute unit
-  const int64_t want = std::max<int64_t>(1, (var_mfma(c) ? 256 : 512) / (tiles * c->n_kv_heads));
-  p->split_pages = (int)std::max<int64_t>(var_mfma(c) ? kSplitPages : kSplitPagesF32, (max_shared + want - 1) / want);
+  // splits of equal pages: as many items as the card takes at once (a workgroup of
+  // the matrix-core kernel per compute unit; of the tile kernel's waves two per SIMD
+  // with 64-wide heads, else one)
+  const int64_t fill = var_mfma(c) ? 256 : d == 64 ? 2048 : 1024;
+  auto split_pages = [&](int64_t t) {
+    const int64_t want = std::max<int64_t>(1, fill / (t * c->n_kv_heads));
+    return (int)std::max<int64_t>(kSplitPages, (max_shared + want - 1) / want);
+  };
+  // matrix-core kernel: tiles of 256 rows (two heads of a sequence per column) where
+  // splits are long and none of these tiles is half empty
+  p->tile_rows = !var_mfma(c) ? 16 : d == 128 && rep > 1 && 2 * wide == tiles && split_pages(tiles) >= kWidePages ? 256 : 128;
+  p->split_pages = split_pages(p->tile_rows == 256 ? wide : tiles);
   for (int i = 0; i < p->n_groups; ++i) {
     const int64_t n = p->g[i].end - p->g[i].first, splits = ceil_div(p->g[i].pages, p->split_pages);
     p->items += ceil_div((int)(n * rep), p->tile_rows) * splits;
@@ -767,19 +690,19 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
     o.prefix.part_ml = x.part_ml;
     const unsigned blocks = (unsigned)(p.items * a.n_kv);
     switch (c->dtype) {
-      case LNSKV_DTYPE_F32: launch_prefix_f32<LNSKV_DTYPE_F32>(x, d, blocks, st); break;
+      case LNSKV_DTYPE_F32: launch_prefix_tile<LNSKV_DTYPE_F32>(x, d, p.items, st); break;
       case LNSKV_DTYPE_F16:
         if (var_mfma(c)) launch_prefix_mfma<false>(x, d, p.tile_rows, blocks, st);
-        else launch_prefix_f32<LNSKV_DTYPE_F16>(x, d, blocks, st);
+        else launch_prefix_tile<LNSKV_DTYPE_F16>(x, d, p.items, st);
         break;
       default:
         if (var_mfma(c)) launch_prefix_mfma<true>(x, d, p.tile_rows, blocks, st);
-        else launch_prefix_f32<LNSKV_DTYPE_Q8A>(x, d, blocks, st);
+        else launch_prefix_tile<LNSKV_DTYPE_Q8A>(x, d, p.items, st);
         break;
     }
     if (int rc = hip_check("prefix kernel launch")) return rc;
   }
-  if (p.shares == 0) return launch_generic<kPrefix>(c, a, p.own, n_seq, ws, o.prefix, st);
+  if (p.shares == 0) return launch_tiles<kPrefix>(c, a, p.own, n_seq, ws, o.prefix, st);
   if (p.shares > 1) {
     o.own_acc = reinterpret_cast<float*>(base + p.own_at);
     o.own_ml = o.own_acc + (size_t)p.shares * n_seq * n_heads * d;

@@ -61,7 +61,7 @@ int sink_sk_waves(int rep, int d, bool q8, int* waves) {
 int plan_sink(const lnskv_pages* c, int n_seq, int n_heads, int64_t units, int64_t pages, VarPlan* p) {
   const int n_kv = (int)c->n_kv_heads, d = (int)c->head_dim, rep = n_heads / n_kv;
   *p = VarPlan{};
-  if (!var_mfma(c)) return plan_generic(c, n_seq, n_heads, pages, p);
+  if (!var_mfma(c)) return plan_tiles(c, n_seq, n_heads, pages, p);
   // the workgroup schedule or stream-K by the size of the batch, as the plain decode
   if (units >= ((int64_t)1 << 30)) return fail(LNSKV_ERR_UNSUPPORTED, "a batch of more than 2^30 page units");
   int n_wg = 0;
@@ -140,7 +140,7 @@ int launch_plan(const lnskv_pages* c, DecodeArgs a, const VarPlan& plan, int64_t
     }
     return LNSKV_OK;
   }
-  return launch_generic<kSink>(c, a, plan, n_seq, ws, x, st);
+  return launch_tiles<kSink>(c, a, plan, n_seq, ws, x, st);
 }
 
 int check_sink(int window, int n_sink) {
