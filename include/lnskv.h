@@ -356,7 +356,8 @@ int lnskv_sink_prefill_attention(const lnskv_pages* c, const float* q_dev, float
  *   attends [0, kv_len_dev[s]), also where that ends inside the shared pages; a
  *   length out of range gives a zero row.  Append the newest tokens first, into
  *   pages that are not shared.  gate_dev (NULL: none) as in
- *   lnskv_gated_append_decode.  workspace_dev / ws_bytes:
+ *   lnskv_gated_append_decode.  Groups on Q8A pages with 128- or 256-wide heads need
+ *   scale arrays under 2 GiB, as lnskv_prefill_attention.  workspace_dev / ws_bytes:
  *   lnskv_prefix_decode_workspace_size bytes (same groups, shape and current
  *   device) or NULL, with lnskv_decode's rules.  Under graph capture the groups
  *   are the captured call's.

@@ -15,8 +15,9 @@ namespace {
 // variant has schedules of its own; on other pages the tile kernel runs in
 // partitions of `split` tokens.
 struct VarPlan {
-  int wg = 0;        // kSink: the workgroup schedule
-  int sk_waves = 0;  // kSink: stream-K
+  bool block = false;  // kSink: a workgroup per (sequence, kv head)
+  int wg = 0;          // kSink: the workgroup schedule
+  int sk_waves = 0;    // kSink: stream-K
   int split = 0;
   int max_parts = 1;
   size_t ws_bytes = 0;

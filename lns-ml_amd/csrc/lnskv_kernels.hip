@@ -1097,8 +1097,12 @@ int lnskv_gated_append_decode(const lnskv_pages* c, const lnskv_rope* rope, cons
 namespace lnskv {
 namespace {
 // Workgroups that share a tile's pairs in the prefill with sinks: as many as fill
-// the compute units (a workgroup takes one whole) while each keeps 16 pairs.
-// 812 queries of 4 x 256-wide Q8A kv heads on 2048 + 16 tokens (104 tiles): SPLIT_US
+// the compute units (a workgroup takes one whole) while each keeps three pairs.
+// 812 queries of 4 x 256-wide Q8A kv heads on 2048 + 16 tokens (104 tiles): 108 us in
+// two splits, the merge among them, 181 unsplit.  Fewest pairs of 16 | 8 | 4 | 2: 2 x up
+// to 189 queries, 8 heads per kv head, up to 992 tokens 72 | 42 | 34 | 34 us; one chunk
+// of 360 on 1457 tokens 48.5 | 33.8 | 29.4 | 27.9; eight of 275 on 125 27.1 | 27.0 | 26.9
+// | 32.1 (the merge of many queries costs more than short chains save).
 int sink_prefill_splits(const lnskv_pages* c, int n_chunks, int n_tok, int bt_stride, int window, int n_sink,
                         int n_heads) {
   const int qt = prefill_queries_per_tile(n_heads / (int)c->n_kv_heads, (int)c->head_dim);
@@ -1106,7 +1110,7 @@ int sink_prefill_splits(const lnskv_pages* c, int n_chunks, int n_tok, int bt_st
   const int64_t all = (int64_t)bt_stride * kPage;
   const int64_t tokens = window > 0 ? std::min(all, (int64_t)window + qt + n_sink) : all;
   const int64_t fill = 256 / std::max<int64_t>(1, tiles * c->n_kv_heads);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({fill, tokens / (16 * 2 * kPage), 16}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({fill, tokens / (3 * 2 * kPage), 16}));
 }
 // The library's decode buffer keeps its header of counts: the rows follow it.
 size_t sink_prefill_bytes(const lnskv_pages* c, int splits, int n_tok, int n_heads) {
@@ -1210,10 +1214,14 @@ int lnskv_sink_prefill_workspace_size(const lnskv_pages* c, int32_t n_chunks, in
   if (!bytes) return fail(LNSKV_ERR_INVALID, "bytes is NULL");
   *bytes = 0;
   if (int rc = check_geometry(c)) return rc;
+  if (n_chunks <= 0 || n_chunks > 65535 || n_tok <= 0 || bt_stride <= 0 || window < 0 || n_sink < 0 || n_sink > (1 << 30))
+    return fail(LNSKV_ERR_INVALID, "n_chunks %d, n_tok %d, bt_stride %d, window %d or n_sink %d out of range", n_chunks,
+                n_tok, bt_stride, window, n_sink);
+  if (n_heads <= 0 || n_heads % (int)c->n_kv_heads != 0)
+    return fail(LNSKV_ERR_INVALID, "n_heads %d is not a multiple of n_kv_heads %u", n_heads, c->n_kv_heads);
   const int rep = n_heads / (int)c->n_kv_heads;
-  if (n_chunks <= 0 || n_tok <= 0 || bt_stride <= 0 || window < 0 || n_sink < 0 || n_sink > (1 << 30) || n_heads <= 0 ||
-      n_heads % (int)c->n_kv_heads != 0 || (rep != 1 && rep != 2 && rep != 4 && rep != 8))
-    return fail(LNSKV_ERR_INVALID, "bad shape");
+  if ((rep != 1 && rep != 2 && rep != 4 && rep != 8) || c->dtype == LNSKV_DTYPE_F32 || c->head_dim == 64)
+    return fail(LNSKV_ERR_UNSUPPORTED, "prefill attention takes f16 and Q8A pages, head_dim 128 or 256, 1, 2, 4 or 8 heads per kv head");
   const int splits = sink_prefill_splits(c, n_chunks, n_tok, bt_stride, window, n_sink, n_heads);
   if (splits > 1) *bytes = sink_prefill_bytes(c, splits, n_tok, n_heads);
   return LNSKV_OK;

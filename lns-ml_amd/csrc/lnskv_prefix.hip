@@ -14,7 +14,7 @@
 //    a sequence with one share merges the prefix's rows and writes its output.
 // 3. join kernel, where sequences may have several shares: their rows and the
 //    prefix's into the output.
-#include "lnskv_decode_mfma.h"
+#include "lnskv_decode_block.h"
 #include "lnskv_decode_var.h"
 #include "lnskv_prefill.h"
 
@@ -406,16 +406,11 @@ __device__ __forceinline__ void merge_rows(const float* acc, const float* ml, si
   for (int c = 0; c < C; ++c) A[c] = A[c] * wa + a2[c] * wb;
 }
 
-constexpr int kOwnWaves = 4;
-
 template <int REP, bool Q8, int NH>
-__global__ __launch_bounds__(kWave* kOwnWaves) __attribute__((amdgpu_waves_per_eu(NH == 1 ? 2 : 1)))
+__global__ __launch_bounds__(kWave* kBlockWaves) __attribute__((amdgpu_waves_per_eu(NH == 1 ? 2 : 1)))
 void prefix_own_kernel(DecodeArgs a, OwnArgs x) {
-  constexpr int NW = kOwnWaves, D = NH * kD, C = D / kWave, kRow = D + 2;
-  constexpr int kSlots = Q8 ? 1 : 2;
-  typedef __attribute__((address_space(3))) float lds_f32;
-  __shared__ __attribute__((aligned(16))) uint8_t vring_[NW][kSlots * NH * kVSlot];
-  __shared__ __attribute__((aligned(16))) float part_[NW * REP * kRow];
+  constexpr int NW = kBlockWaves, D = NH * kD, C = D / kWave;
+  __shared__ BlockLds<REP, Q8, NH> sm;
   const int wi = (int)(threadIdx.x / kWave), lane = (int)(threadIdx.x % kWave);
   // share slowest: the first shares, which every sequence has, start first
   const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
@@ -427,39 +422,13 @@ void prefix_own_kernel(DecodeArgs a, OwnArgs x) {
   // wave w: pages [lo + w per, lo + (w + 1) per) of the sequence's own
   const int per = ceil_div(hi - lo, NW);
   const int i0 = min(hi, lo + wi * per), i1 = min(hi, i0 + per);
-  if (i0 < i1) {
-    const int pg0 = o.p0 / kPage;
-    PieceLoads<REP, NH> pl;
-    piece_loads<REP, false, false, Q8, NH>(a, s, kvh, pg0 + i0, pl);
-    PieceOut po;
-    po.final = false;
-    po.pbase = (size_t)wi * REP;
-    po.pstride = 1;
-    po.in_lds = true;
-    po.lds = (lds_f32*)part_;
-    if constexpr (Q8)
-      run_piece_q8<REP, 2, false, NH, false>(a, (lds_u8*)vring_[wi], (lds_u8*)vring_[wi], pl, true, s, kvh,
-                                             (pg0 + i0) * kPage, min(o.L, (pg0 + i1) * kPage), false, o.L - 1, po, nullptr);
-    else
-      run_piece<REP, false, 2, false, NH>(a, (lds_u8*)vring_[wi], (lds_u8*)vring_[wi], pl, true, s, kvh,
-                                          (pg0 + i0) * kPage, min(o.L, (pg0 + i1) * kPage), false, o.L - 1, po, nullptr);
-  }
+  if (i0 < i1) block_piece<REP, Q8, NH>(a, sm, wi, s, kvh, o.p0 / kPage, i0, i1, o.L);
   __syncthreads();
   const int nw = hi > lo ? ceil_div(hi - lo, per) : 0;  // waves that left rows
   for (int h = wi; h < REP; h += NW) {  // wave-uniform
     const size_t hrow = (size_t)s * a.n_heads + (size_t)kvh * REP + h;
-    float M = kMInit, Ls = 0.0f, A[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) A[c] = 0.0f;
-    for (int w = 0; w < nw; ++w) {
-      const lds_f32* row = (const lds_f32*)part_ + ((size_t)w * REP + h) * kRow;
-      const float m = row[D], Mn = fmaxf(M, m);
-      const float wa = fast_exp2(M - Mn), wb = fast_exp2(m - Mn);
-      Ls = Ls * wa + row[D + 1] * wb;
-#pragma unroll
-      for (int c = 0; c < C; ++c) A[c] = A[c] * wa + row[lane + c * kWave] * wb;
-      M = Mn;
-    }
+    float M, Ls, A[C];
+    block_merge<REP, Q8, NH>(sm, nw, h, M, Ls, A);
     if (o.shares == 1) {
       merge_rows<D>(x.prefix.part_acc, x.prefix.part_ml, o.prefix.base + (size_t)(kvh * REP + h) * o.prefix.splits,
                     o.prefix.splits, M, Ls, A);
@@ -507,10 +476,10 @@ __global__ __launch_bounds__(kBlock) void prefix_join_kernel(DecodeArgs a, OwnAr
 template <bool Q8, int NH>
 void launch_own_rep(const DecodeArgs& a, const OwnArgs& x, int rep, unsigned blocks, hipStream_t st) {
   switch (rep) {
-    case 1: prefix_own_kernel<1, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
-    case 2: prefix_own_kernel<2, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
-    case 4: prefix_own_kernel<4, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
-    default: prefix_own_kernel<8, Q8, NH><<<blocks, kWave * kOwnWaves, 0, st>>>(a, x); break;
+    case 1: prefix_own_kernel<1, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
+    case 2: prefix_own_kernel<2, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
+    case 4: prefix_own_kernel<4, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
+    default: prefix_own_kernel<8, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
   }
 }
 
@@ -647,6 +616,10 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
   if (int rc = check_var_shape(c, n_seq, n_heads, max_kv_len)) return rc;
   PrefixPlan p;
   if (int rc = plan_prefix(c, groups, n_groups, n_seq, n_heads, max_kv_len, &p)) return rc;
+  if (p.n_groups > 0 && var_mfma(c) && c->dtype == LNSKV_DTYPE_Q8A &&
+      (uint64_t)c->num_pages * kPage * c->n_kv_heads * sizeof(float) > 0x7FFFFFF0u)  // the page pipeline's scale offsets
+    return fail(LNSKV_ERR_UNSUPPORTED, "shared prefixes on Q8A pages need scale arrays under 2 GiB (%u pages x %u kv heads)",
+                c->num_pages, c->n_kv_heads);
   const hipStream_t st = (hipStream_t)stream;
   if (int rc = var_workspace(&ws, ws_bytes, p.ws_bytes, st)) return rc;
   const DecodeArgs a = var_args(c, q, out, gate, bt, bt_stride, kv_len, n_heads, max_kv_len, scale, p.own, stream);

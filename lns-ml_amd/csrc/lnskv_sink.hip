@@ -6,13 +6,50 @@
 // entry), so that every schedule divides exactly the pages that are read; a
 // page that holds both attended and other tokens is masked token by token.
 // Bound by HBM like the plain decode: sinks + window tokens of K and V.
-#include "lnskv_decode_mfma.h"
+#include "lnskv_decode_block.h"
 #include "lnskv_decode_var.h"
 
 namespace lnskv {
 namespace {
 
 constexpr int kMaxSink = 1 << 30;
+// Pages of a sequence up to which one workgroup per (sequence, kv head) takes them all,
+// and up to which it does where those workgroups are about as many as compute units.
+// Us, that | the plain decode's schedules: 17 sequences x 4 kv heads, window 84 + 61, Q8A
+// 9.4 | 15.6; 16 x 4, 281 + 61, f16 8.9 | 12.9; 1 x 8, 102 + 55, f16 7.8 | 11.7; 18 x 4
+// 256-wide, 182 + 58, Q8A 16.7 | 18.1; 60 x 4, 854 + 4, Q8A 18.4 | 23.2; but 6 x 4, 873 +
+// 39, Q8A 19.0 | 12.2 and 1 x 8, 1024 + 4, Q8A 20.3 | 13.7.
+constexpr int kBlockPages = 32;
+constexpr int kBlockPagesFull = 64;
+
+// A workgroup per (sequence, kv head): bound by the latency of its four waves' chains
+// of at most 16 pages each.
+template <int REP, bool Q8, int NH>
+__global__ __launch_bounds__(kWave* kBlockWaves) __attribute__((amdgpu_waves_per_eu(NH == 1 ? 2 : 1)))
+void sink_block_kernel(DecodeArgs a, VarArgs<kSink> x) {
+  constexpr int NW = kBlockWaves, D = NH * kD, C = D / kWave;
+  __shared__ BlockLds<REP, Q8, NH> sm;
+  const int wi = (int)(threadIdx.x / kWave), lane = (int)(threadIdx.x % kWave);
+  const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv), s = (int)(blockIdx.x / (unsigned)a.n_kv);
+  int L = a.kv_len[s];
+  L = L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : max(L, 0);
+  const SinkSpan sp = sink_span(x, L);
+  const int np = L > 0 ? (L - 1) / kPage + 1 - sp.gap : 0;
+  const int per = (np + NW - 1) / NW, i0 = min(np, wi * per), i1 = min(np, i0 + per);
+  if (i0 < i1) block_piece<REP, Q8, NH, kSink>(a, sm, wi, s, kvh, 0, i0, i1, L, sp);
+  __syncthreads();
+  const int nw = np > 0 ? (np + per - 1) / per : 0;  // waves that left rows
+  for (int h = wi; h < REP; h += NW) {  // wave-uniform
+    float M, Ls, A[C];
+    block_merge<REP, Q8, NH>(sm, nw, h, M, Ls, A);
+    const size_t row = ((size_t)s * a.n_heads + (size_t)kvh * REP + h) * D;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const size_t i = row + c * kWave + lane;
+      a.out[i] = gated(a, i, Ls > 0.0f ? A[c] / Ls : 0.0f);
+    }
+  }
+}
 
 int64_t sink_pages(int max_kv_len, int window, int n_sink) {
   const int64_t all = (int64_t)max_kv_len / kPage + 1;
@@ -62,6 +99,10 @@ int plan_sink(const lnskv_pages* c, int n_seq, int n_heads, int64_t units, int64
   const int n_kv = (int)c->n_kv_heads, d = (int)c->head_dim, rep = n_heads / n_kv;
   *p = VarPlan{};
   if (!var_mfma(c)) return plan_tiles(c, n_seq, n_heads, pages, p);
+  if (pages <= ((int64_t)n_seq * n_kv >= 192 ? kBlockPagesFull : kBlockPages)) {
+    p->block = true;
+    return LNSKV_OK;
+  }
   // the workgroup schedule or stream-K by the size of the batch, as the plain decode
   if (units >= ((int64_t)1 << 30)) return fail(LNSKV_ERR_UNSUPPORTED, "a batch of more than 2^30 page units");
   int n_wg = 0;
@@ -103,6 +144,16 @@ int launch_plan(const lnskv_pages* c, DecodeArgs a, const VarPlan& plan, int64_t
   const int d = (int)c->head_dim, rep = a.n_heads / a.n_kv;
   const bool q8 = c->dtype == LNSKV_DTYPE_Q8A;
   uint8_t* body = static_cast<uint8_t*>(ws) + (ws ? kWsHeaderBytes : 0);
+  if (plan.block) {
+    const unsigned blocks = (unsigned)(n_seq * a.n_kv);
+    if (int rc = with_rep_nh(rep, d, [&](auto rep_c, auto nh_c) {
+          constexpr int R = decltype(rep_c)::value, NH = decltype(nh_c)::value;
+          if (q8) sink_block_kernel<R, true, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x);
+          else sink_block_kernel<R, false, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x);
+        }))
+      return rc;
+    return hip_check("decode kernel launch");
+  }
   if (plan.wg > 0) {
     a.wg_cnt = static_cast<uint32_t*>(ws);
     a.ws_acc = reinterpret_cast<float*>(body);

@@ -172,7 +172,10 @@ def test_prefill_without_sinks_is_the_windowed_prefill():
     for window in (0, 90):
         a = pk.prefill_attention(q, ch, t, n_heads=8, scale=0.1, window=window)
         b = pk.sink_prefill_attention(q, ch, t, n_heads=8, scale=0.1, window=window, n_sink=0)
-        assert torch.equal(a, b)
+        if pk.sink_prefill_workspace_size(1, 300, 25, window, 0, 8) == 0:
+            assert torch.equal(a, b)
+        else:  # split along the keys: both are within TOL of the exact result, so within 2 TOL of each other
+            assert window == 0 and A.worst(b, a.cpu().numpy()) < 2 * A.TOL
 
 
 def test_prefill_skips_chunks_outside_the_inputs():
@@ -189,7 +192,8 @@ def test_prefill_skips_chunks_outside_the_inputs():
     assert touched[8:16].all() and not touched[:8].any() and not touched[16:].any()
 
 
-def test_decode_captured_and_replayed():
+@pytest.mark.parametrize("window", [100, 800])
+def test_decode_captured_and_replayed(window):
     """A captured call replayed over changed inputs, with eager work between."""
     rng = np.random.default_rng(6)
     lens = [900, 40, 333]
@@ -198,10 +202,10 @@ def test_decode_captured_and_replayed():
     A.fill(pk, 3)
     q = dev_f32(rng.standard_normal((3, 8, 128)), DEV)
     t, kl = dev_i32(tables, DEV), dev_i32(np.array(lens, np.int32), DEV)
-    ws = torch.zeros(pk.sink_workspace_size(3, 8, 900, 100, 4), dtype=torch.uint8, device=DEV)
+    ws = torch.zeros(pk.sink_workspace_size(3, 8, 900, window, 4), dtype=torch.uint8, device=DEV)
     eager_ws = torch.zeros_like(ws)
     out = torch.empty((3, 8, 128), device=DEV)
-    call = dict(n_heads=8, max_kv_len=900, scale=0.1, window=100, n_sink=4)
+    call = dict(n_heads=8, max_kv_len=900, scale=0.1, window=window, n_sink=4)
     pk.sink_decode(q, t, kl, workspace=ws, out=out, **call)
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
@@ -216,24 +220,26 @@ def test_decode_captured_and_replayed():
         assert torch.equal(out, want)
 
 
-def test_decode_on_another_stream_and_wrong_inputs():
+@pytest.mark.parametrize("window", [50, 1000])
+def test_decode_on_another_stream_and_wrong_inputs(window):
     rng = np.random.default_rng(7)
     tables, n = A.make_tables([200], [range(13)], rng)
     pk = PagedKV(n, 2, 128, DTYPE_F16, DEV)
     A.fill(pk, 3)
     q = dev_f32(rng.standard_normal((1, 8, 128)), DEV)
     t, kl = dev_i32(tables, DEV), dev_i32(np.array([200], np.int32), DEV)
-    call = dict(n_heads=8, max_kv_len=200, scale=0.1, window=50, n_sink=4)
+    call = dict(n_heads=8, max_kv_len=208, scale=0.1, window=window, n_sink=4)
     want = pk.sink_decode(q, t, kl, **call)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
-        ws = torch.zeros(pk.sink_workspace_size(1, 8, 200, 50, 4), dtype=torch.uint8, device=DEV)
+        ws = torch.zeros(pk.sink_workspace_size(1, 8, 208, window, 4), dtype=torch.uint8, device=DEV)
         got = pk.sink_decode(q, t, kl, workspace=ws, **call)
     s.synchronize()
     assert torch.equal(got, want)
-    with pytest.raises(LnskvError):
-        pk.sink_decode(q, t, kl, workspace=torch.zeros(16, dtype=torch.uint8, device=DEV), **call)
+    with pytest.raises(LnskvError):  # more tokens than one workgroup takes
+        pk.sink_decode(q, t, kl, workspace=torch.zeros(16, dtype=torch.uint8, device=DEV),
+                       **dict(call, max_kv_len=9000, window=5000))
     with pytest.raises(ValueError):
         pk.sink_decode(q.transpose(1, 2), t, kl, **call)
     with pytest.raises(TypeError):

@@ -110,6 +110,35 @@ def test_prefix_decode_refuses(kw, rc, text):
     assert got == rc and text in msg, (got, msg)
 
 
+def test_prefix_decode_of_large_q8a_pools():
+    """2^22 pages x 8 kv heads: 2 GiB of scales, past the page pipeline's 32-bit offsets."""
+    big = pages(_lib.DTYPE_Q8A, 128, kv=8, n=1 << 22)
+    got, msg = prefix(c=big, n_heads=8)
+    assert got == UNS and "2 GiB" in msg
+    for ok in (pages(_lib.DTYPE_Q8A, 128, kv=8, n=(1 << 22) - 1), pages(_lib.DTYPE_F16, 128, kv=8, n=1 << 22),
+               pages(_lib.DTYPE_Q8A, 64, kv=8, n=1 << 22)):
+        got, msg = prefix(c=ok, n_heads=8, ws_bytes=16)  # further checks come after
+        assert got == WS and "needed" in msg
+
+
+def test_sink_prefill_workspace_query():
+    lib, out = _lib.lib(), C.c_size_t(7)
+
+    def size(c, n_chunks=1, n_tok=64, stride=512, window=4096, n_sink=4, n_heads=8):
+        rc = lib.lnskv_sink_prefill_workspace_size(C.byref(c), n_chunks, n_tok, stride, window, n_sink, n_heads,
+                                                   C.byref(out))
+        return rc, out.value
+    f16 = pages(_lib.DTYPE_F16, 128)
+    assert lib.lnskv_sink_prefill_workspace_size(C.byref(f16), 1, 64, 512, 4096, 4, 8, None) == INV
+    for kw in (dict(window=-1), dict(n_sink=-1), dict(n_heads=6)):
+        assert size(f16, **kw) == (INV, 0)
+    assert size(pages(d=128)) == (UNS, 0) and size(pages(_lib.DTYPE_F16, 64)) == (UNS, 0)
+    rc, few = size(f16)  # 64 queries on 4096 tokens: split, a row per query head and split
+    assert rc == 0 and few >= 2 * 64 * 8 * (128 + 2) * 4
+    assert size(f16, n_tok=1 << 20) == (0, 0)  # tiles enough for every compute unit
+    assert size(f16, stride=2) == (0, 0)  # one pair of pages
+
+
 def test_sink_prefill_refuses():
     def call(c, window=16, n_sink=4, n_heads=8, chunks=P):
         return status("lnskv_sink_prefill_attention", C.byref(c), P, P, chunks, 1, 4, P, 4, 1, window, n_sink, n_heads, 0.1,
