@@ -99,7 +99,8 @@ int plan_sink(const lnskv_pages* c, int n_seq, int n_heads, int64_t units, int64
   const int n_kv = (int)c->n_kv_heads, d = (int)c->head_dim, rep = n_heads / n_kv;
   *p = VarPlan{};
   if (!var_mfma(c)) return plan_tiles(c, n_seq, n_heads, pages, p);
-  if (pages <= ((int64_t)n_seq * n_kv >= 192 ? kBlockPagesFull : kBlockPages)) {
+  const int setting = schedule_setting();
+  if (setting == kScheduleAuto && pages <= ((int64_t)n_seq * n_kv >= 192 ? kBlockPagesFull : kBlockPages)) {
     p->block = true;
     return LNSKV_OK;
   }
@@ -107,7 +108,6 @@ int plan_sink(const lnskv_pages* c, int n_seq, int n_heads, int64_t units, int64
   if (units >= ((int64_t)1 << 30)) return fail(LNSKV_ERR_UNSUPPORTED, "a batch of more than 2^30 page units");
   int n_wg = 0;
   if (int rc = mfma_wg_count(&n_wg)) return rc;
-  const int setting = schedule_setting();
   if (n_seq <= kSkMaxSeqs &&
       (setting == kScheduleWorkgroup || (setting == kScheduleAuto && units <= (int64_t)kWgSmallPages * n_wg))) {
     p->wg = n_wg;

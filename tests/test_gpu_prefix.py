@@ -128,6 +128,62 @@ def test_more_sequences_than_a_launch_takes(dtype):
     assert case(dtype, 128, 1, 1, groups, lens, seed=8) < A.TOL
 
 
+@pytest.mark.parametrize("dtype", [DTYPE_F16, DTYPE_Q8A])
+@pytest.mark.parametrize("kv,rep,n", [(32, 2, 128), (8, 8, 160)])
+def test_long_prefixes_of_many_rows(dtype, kv, rep, n):
+    """Tiles of 256 rows (the last one partly empty or not), against the plain decode:
+    each is within TOL of the exact result, so they are within 2 TOL of each other."""
+    say("prefix wide", dtype, kv, rep, n)
+    rng = np.random.default_rng(13)
+    tok, H = 3200, kv * rep
+    tables = np.full((n, 202), 0xFFFFFFFF, np.uint32)
+    order = rng.permutation(200 + 2 * n + 1)
+    tables[:, :200] = order[:200]
+    tables[:, 200:] = order[200:200 + 2 * n].reshape(n, 2)
+    lens = tok + rng.integers(0, 33, n)
+    lens[[3, n - 1]] = [1777, 0]
+    pk = PagedKV(len(order), kv, 128, dtype, DEV)
+    A.fill(pk, 13)
+    q, t, kl = dev_f32(rng.standard_normal((n, H, 128)), DEV), dev_i32(tables, DEV), dev_i32(lens.astype(np.int32), DEV)
+    call = dict(n_heads=H, max_kv_len=3232, scale=0.1)
+    want = pk.decode(q, t, kl, **call)
+    got = pk.prefix_decode(q, t, kl, PrefixGroups([(0, n, tok)]), **call)
+    assert A.worst(got, want.cpu().numpy().astype(np.float64)) < 2 * A.TOL
+
+
+def test_two_calls_at_once():
+    """Prefixes and sinks on two streams with workspaces of their own, as one after the other."""
+    rng = np.random.default_rng(14)
+    lens = [900, 877, 850, 1100]
+    tables, n = A.make_tables([1100] * 4, [range(69)] * 4, rng)
+    tables[1:, :50] = tables[0, :50]
+    pk = PagedKV(n, 4, 128, DTYPE_Q8A, DEV)
+    A.fill(pk, 3)
+    q, t, kl = dev_f32(rng.standard_normal((4, 16, 128)), DEV), dev_i32(tables, DEV), dev_i32(np.array(lens, np.int32), DEV)
+    plan, call = PrefixGroups([(0, 4, 800)]), dict(n_heads=16, max_kv_len=1100, scale=0.1)
+    chunks, pq = dev_i32(np.array([[0, 860, 40, 0]], np.int32), DEV), dev_f32(rng.standard_normal((40, 16, 128)), DEV)
+    sizes = [pk.prefix_workspace_size(plan, 4, 16, 1100), pk.sink_workspace_size(4, 16, 1100, 1000, 4),
+             pk.sink_prefill_workspace_size(1, 40, 69, 700, 4, 16)]
+    assert min(sizes) > 0
+
+    def all_of(ws):
+        return [pk.prefix_decode(q, t, kl, plan, workspace=ws[0], **call),
+                pk.sink_decode(q, t, kl, window=1000, n_sink=4, workspace=ws[1], **call),
+                pk.sink_prefill_attention(pq, chunks, t, n_heads=16, scale=0.1, window=700, n_sink=4, workspace=ws[2])]
+    spaces = [[torch.zeros(x, dtype=torch.uint8, device=DEV) for x in sizes] for _ in range(2)]
+    want = all_of(spaces[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, ws in zip(streams, spaces):
+            with torch.cuda.stream(s):
+                got.append(all_of(ws))
+        torch.cuda.synchronize()
+        for outs in got:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 def test_no_groups_is_the_plain_decode():
     rng = np.random.default_rng(9)
     lens = [50, 300, 7]
