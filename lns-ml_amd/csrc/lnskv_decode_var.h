@@ -23,7 +23,12 @@ struct VarPlan {
   size_t ws_bytes = 0;
 };
 
-constexpr int kOnePartition = 256;  // tokens
+// Tokens of a sequence up to which one block takes them all, and the fewest that a
+// partition has otherwise.  Us: 7 sequences x 8 kv heads of 240 tokens, Q8A, 64-wide: one
+// block 7.7, partitions of 64 10.7, of 128 10.2 (a second launch merges); 24 x 4 of 1021,
+// f32: of 64 16.6, 128 15.3, 192 17.5, 256 15.8, 512 19.5; 3 x 4 of 3700, Q8A: 12.3, 11.0,
+// 10.9, 11.6, 16.2.
+constexpr int kOnePartition = 256;
 constexpr int kLeastPartition = 128;
 
 inline bool var_mfma(const lnskv_pages* c) {

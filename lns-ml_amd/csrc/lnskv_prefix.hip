@@ -30,8 +30,16 @@ constexpr int kSplitPages = 2;
 // (splits of 32 pages) 42.9 | 45.3, 8000 66.2 | 62.6, 16000 109 | 100; Q8A 51.3 | 50.8,
 // 78.2 | 70.9, 125 | 111.
 constexpr int kWidePages = 48;
-constexpr int kSharePages = 64;  // most pages of a share of a sequence's own
+// A sequence's own pages: shares of at most kSharePages pages (four waves, 16 each).
+// Batches that leave compute units idle take smaller ones, but for short ones
+// (kShareWhole pages), where the rows' way through memory and the join cost more: 48 x 4
+// kv heads of up to 300 tokens, Q8A, 256-wide, in all 44.5 us whole and 54.8 in shares of
+// kShareMin; 4 x 8 of up to 1000 tokens, f16, 21.0 in shares and 24.3 whole.  kSharePages
+// 32 | 64 | 128, 64 x 8 of up to 4000 tokens: 165 | 165 | 171 us.  kShareMin 4 | 8 | 16, 4
+// x 8 of up to 1000: 23.0 | 21.0 | 21.5.
+constexpr int kSharePages = 64;
 constexpr int kShareMin = 8;
+constexpr int kShareWhole = 32;
 
 struct PrefixArgs {
   PrefillArgs pf;  // the pools, for the prefill kernel's page pipeline
@@ -104,6 +112,10 @@ __device__ __forceinline__ int row_tokens(const PrefixArgs& a, int s, int pages)
 // f32 pages, and 64-wide heads on every page type, in f32 (lnskv_decode_tile.h): a
 // wave per item of 16 rows and one split.  The waves of a block take the tiles of
 // one split, or consecutive splits of few rows, and share nothing but the cache.
+// Bound by the products (v_mfma_f32_16x16x4_f32, 32 cycles) once groups are large: 109
+// sequences x 2 heads on 8 of 128 behind 4407 tokens, f32, 59 us in all (28 at the
+// library's f32 rate), 68 with the page shared by four waves in LDS; by latency where they
+// are small: 2 sequences x 8 heads on 4 of 64 behind 256 tokens 6.3 us.
 template <int DT, int D>
 __global__ __launch_bounds__(kBlock) void prefix_tile_kernel(PrefixArgs a) {
   const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
@@ -169,6 +181,11 @@ __global__ __launch_bounds__(kBlock) void prefix_tile_kernel(PrefixArgs a) {
 // HW)) ..), so that its HW rows have the same length.  HW = 2 shares each K and V
 // operand read from LDS between two rows' tiles (NH = 1; a 256-wide head's
 // accumulators leave room for one).
+// Bound by its chain of LDS reads, products and softmax per pair of pages, two waves to a
+// SIMD; short splits by latency and the partial rows' bytes.  128 sequences x 4 heads on 8
+// behind 16384 tokens, f16: 85 to 89 us (34 GFLOP, twice that in products of hi and lo
+// parts: 59 us at the rate of a large library product); 3 x 16 sequences x 4 heads on 4 of
+// 256 behind 4090 tokens, Q8A: 26 us; 32 x 4 on 8 behind 2048, f16: 12.6 us.
 template <bool Q8, int NH, int HW>
 __global__ __launch_bounds__(kWave * 8) void prefix_mfma_kernel(PrefixArgs a) {
   constexpr int D = NH * kD, NW = 8;
@@ -365,7 +382,10 @@ __global__ __launch_bounds__(kWave * 8) void prefix_mfma_kernel(PrefixArgs a) {
 // share_pages pages) of one (sequence, kv head); its four waves split the share
 // and stream their pages as the decode kernels do, each by itself (K to registers,
 // V through an LDS ring, two pages in flight), leave partial rows in LDS, and
-// merge them head by head.  No workgroup depends on another.
+// merge them head by head.  No workgroup depends on another.  Bound by HBM in large
+// batches: 128 sequences x 8 kv heads of 64 to 1024 tokens, f16, with the prefix's 16
+// partial rows per head: 84 us (318 MB: 66 at a large copy's rate; three waves to a SIMD
+// instead of two spill and take 94); 32 of up to 512 12 to 15.
 struct OwnArgs {
   VarArgs<kPrefix> prefix;
   float* own_acc;  // [n_seq][n_heads][shares][D], where a sequence has several shares
@@ -551,7 +571,7 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   if (var_mfma(c)) {
     // shares of at most kSharePages pages, fewer where that leaves compute units idle
     const int64_t units = own_pages * c->n_kv_heads;
-    p->share_pages = n_seq * (int64_t)c->n_kv_heads >= 256 || most <= 32
+    p->share_pages = n_seq * (int64_t)c->n_kv_heads >= 256 || most <= kShareWhole
                          ? kSharePages
                          : (int)std::min<int64_t>(kSharePages, std::max<int64_t>(kShareMin, (units + 511) / 512));
     p->shares = (int)std::max<int64_t>(1, (most + p->share_pages - 1) / p->share_pages);
