@@ -323,7 +323,10 @@ int lnskv_mrope_append(const lnskv_pages* c, const lnskv_rope* rope, const int32
  * lnskv_sink_prefill_workspace_size bytes, 0 where nothing is split; a smaller one
  * is not used and nothing is split; no header to zero) or, where that is NULL, in the
  * library's decode buffer (calls that use it must not overlap in time; while a
- * stream is captured it is used only if it is large enough already).
+ * stream is captured it is used only if it is large enough already).  Slots that no
+ * query attends may hold any bits; a K or V value that is not finite at a token that some
+ * query of a tile attends may reach the tile's other queries, as in
+ * lnskv_prefill_attention.
  * ------------------------------------------------------------------------- */
 int lnskv_sink_decode_workspace_size(const lnskv_pages* c, int32_t n_seq, int32_t n_heads,
                                      int32_t max_kv_len, int32_t window, int32_t n_sink, size_t* bytes);
@@ -357,7 +360,10 @@ int lnskv_sink_prefill_attention(const lnskv_pages* c, const float* q_dev, float
  *   length out of range gives a zero row.  Append the newest tokens first, into
  *   pages that are not shared.  gate_dev (NULL: none) as in
  *   lnskv_gated_append_decode.  Groups on Q8A pages with 128- or 256-wide heads need
- *   scale arrays under 2 GiB, as lnskv_prefill_attention.  workspace_dev / ws_bytes:
+ *   scale arrays under 2 GiB, as lnskv_prefill_attention.  Slots that no sequence
+ *   attends may hold any bits; a value that is not finite at a shared token may reach
+ *   every sequence of the group, also one whose length ends before it.  workspace_dev /
+ *   ws_bytes:
  *   lnskv_prefix_decode_workspace_size bytes (same groups, shape and current
  *   device) or NULL, with lnskv_decode's rules.  Under graph capture the groups
  *   are the captured call's.
