@@ -19,12 +19,11 @@ struct BlockLds {
 };
 
 // Wave wi's row of partial results of pages [i0, i1), counted from page pg0; tokens
-// from L on are masked (kSink: what the span does not see).
+// from L on are masked (kSink: what the span does not see).  pl: piece_loads of the
+// first of them.
 template <int REP, bool Q8, int NH, int VAR = kPlain, class... SP>
 __device__ __forceinline__ void block_piece(const DecodeArgs& a, BlockLds<REP, Q8, NH>& sm, int wi, int s, int kvh,
-                                            int pg0, int i0, int i1, int L, const SP&... sp) {
-  PieceLoads<REP, NH> pl;
-  piece_loads<REP, false, false, Q8, NH, VAR>(a, s, kvh, pg0 + i0, pl, sp...);
+                                            PieceLoads<REP, NH>& pl, int pg0, int i0, int i1, int L, const SP&... sp) {
   PieceOut po;
   po.final = false;
   po.pbase = (size_t)wi * REP;

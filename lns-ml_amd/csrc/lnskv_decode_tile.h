@@ -223,7 +223,12 @@ __global__ __launch_bounds__(kBlock) void decode_tile_kernel(DecodeArgs a, VarAr
     return pg;
   };
   const int pg0 = ta / kPage, pages = ta < tb ? (tb - 1) / kPage + 1 - pg0 : 0;  // at most 64
-  const uint32_t btv = lane < pages ? a.bt[(size_t)s * a.bt_stride + entry(pg0 + lane)] : 0xFFFFFFFFu;
+  int row = s;
+  if constexpr (VAR == kPrefix) {
+    const PrefixRows pr = prefix_rows(x, s, a.n_heads);
+    row = pg0 + lane < pr.pages ? pr.first : s;
+  }
+  const uint32_t btv = lane < pages ? a.bt[(size_t)row * a.bt_stride + entry(pg0 + lane)] : 0xFFFFFFFFu;
   TileState<DT, D> st;
   tile_init<DT, D>(st, a.q + ((size_t)s * a.n_heads + kvh * REP + n % REP) * D, a.scale_log2, g);
   tile_pages<DT, D>(

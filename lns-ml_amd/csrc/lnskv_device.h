@@ -276,26 +276,28 @@ struct PrefixGroup {
 template <> struct VarArgs<kPrefix> {
   const float* part_acc;  // partial rows of the groups' prefixes: numerators,
   const float* part_ml;   // running max (log2 units) and sum
-  int32_t split_pages;    // a group's pages are split every so many
+  int32_t split_pages;    // a group's pages are split every so many; 0: no such rows, every
+                          // sequence reads the shared pages itself
   int32_t n_groups;
   PrefixGroup g[LNSKV_PREFIX_MAX_GROUPS];
 };
 
-// The shared pages of sequence s (0 where it is in no group) and its prefix's
-// partial rows: head h has rows base + h * splits .. + splits - 1.
+// The shared pages of sequence s (0 where it is in no group), the table row they are
+// taken from, and its prefix's partial rows: head h has rows base + h * splits .. +
+// splits - 1.
 struct PrefixRows {
   size_t base;
-  int splits, pages;
+  int splits, pages, first;
 };
 __device__ __forceinline__ PrefixRows prefix_rows(const VarArgs<kPrefix>& x, int s, int n_heads) {
   size_t at = 0;
   for (int i = 0; i < x.n_groups; ++i) {
     const PrefixGroup g = x.g[i];
-    const int splits = (g.pages + x.split_pages - 1) / x.split_pages;
-    if (s >= g.first && s < g.end) return {at + (size_t)(s - g.first) * n_heads * splits, splits, g.pages};
+    const int splits = x.split_pages > 0 ? (g.pages + x.split_pages - 1) / x.split_pages : 0;
+    if (s >= g.first && s < g.end) return {at + (size_t)(s - g.first) * n_heads * splits, splits, g.pages, g.first};
     at += (size_t)(g.end - g.first) * n_heads * splits;
   }
-  return {0, 0, 0};
+  return {0, 0, 0, s};
 }
 
 // kSink: the attended tokens of a sequence are t < n_sink and p0 <= t < L.
@@ -352,7 +354,7 @@ __device__ __forceinline__ SeqWindow seq_window(const DecodeArgs& a, int s, cons
   }
   int p0 = a.p_start ? a.p_start[s] : a.p_start_scalar;
   if constexpr (VAR == kPrefix) {  // partitions from the prefix's end on
-    p0 = min(prefix_rows(only(x...), s, a.n_heads).pages * kPage, L);
+    p0 = only(x...).split_pages > 0 ? min(prefix_rows(only(x...), s, a.n_heads).pages * kPage, L) : 0;
     w.L = L;
     w.p0 = p0;
     w.jf = 0;

@@ -14,6 +14,8 @@
 //    a sequence with one share merges the prefix's rows and writes its output.
 // 3. join kernel, where sequences may have several shares: their rows and the
 //    prefix's into the output.
+// Short sequences take one launch instead, in which each reads its group's pages
+// itself (block kernel, or the tile kernel).
 #include "lnskv_decode_block.h"
 #include "lnskv_decode_var.h"
 #include "lnskv_prefill.h"
@@ -40,6 +42,17 @@ constexpr int kWidePages = 48;
 constexpr int kSharePages = 64;
 constexpr int kShareMin = 8;
 constexpr int kShareWhole = 32;
+// Sequences of at most kDirectPages pages (half of that with 128- and 256-wide f32 heads,
+// whose f32 products take longest) and kDirectBytes of K and V, shared pages counted
+// every time, are decoded in one launch in which each reads its group's pages itself, from
+// L2 mostly.  Us, one launch | prefix and own pages apart, sequences x kv heads of pages:
+// f16 128-wide 4 x 8 of 13 7.3 | 13.8, 16 x 8 of 57 13.3 | 19.2, 64 x 8 of 57 (228 MB) 22.3
+// | 26.4, 128 x 8 of 57 (456 MB) 42.6 | 39.9, 16 x 8 of 107 20.8 | 21.2, 64 x 8 of 107 37 |
+// 28.5; Q8A 128 x 8 of 57 (228 MB) 39.4 | 36.7, 256-wide 64 x 4 of 26 17.4 | 26.6; f32
+// 64-wide 2 x 4 of 21 8.8 | 12.6, 128-wide 64 x 8 of 13 (104 MB) 17.0 | 22.2, of 26 (208 MB)
+// 26.8 | 23.2, 4 x 8 of 57 23.2 | 20.7.
+constexpr int kDirectPages = 64;
+constexpr int64_t kDirectBytes = (int64_t)192 << 20;
 
 struct PrefixArgs {
   PrefillArgs pf;  // the pools, for the prefill kernel's page pipeline
@@ -442,7 +455,11 @@ void prefix_own_kernel(DecodeArgs a, OwnArgs x) {
   // wave w: pages [lo + w per, lo + (w + 1) per) of the sequence's own
   const int per = ceil_div(hi - lo, NW);
   const int i0 = min(hi, lo + wi * per), i1 = min(hi, i0 + per);
-  if (i0 < i1) block_piece<REP, Q8, NH>(a, sm, wi, s, kvh, o.p0 / kPage, i0, i1, o.L);
+  if (i0 < i1) {
+    PieceLoads<REP, NH> pl;
+    piece_loads<REP, false, false, Q8, NH>(a, s, kvh, o.p0 / kPage + i0, pl);
+    block_piece<REP, Q8, NH>(a, sm, wi, s, kvh, pl, o.p0 / kPage, i0, i1, o.L);
+  }
   __syncthreads();
   const int nw = hi > lo ? ceil_div(hi - lo, per) : 0;  // waves that left rows
   for (int h = wi; h < REP; h += NW) {  // wave-uniform
@@ -465,6 +482,40 @@ void prefix_own_kernel(DecodeArgs a, OwnArgs x) {
         x.own_ml[2 * r] = M;
         x.own_ml[2 * r + 1] = Ls;
       }
+    }
+  }
+}
+
+// Short sequences: a workgroup per (sequence, kv head) takes the shared pages and its own
+// in one launch.
+template <int REP, bool Q8, int NH>
+__global__ __launch_bounds__(kWave* kBlockWaves) __attribute__((amdgpu_waves_per_eu(NH == 1 ? 2 : 1)))
+void prefix_block_kernel(DecodeArgs a, VarArgs<kPrefix> x) {
+  constexpr int NW = kBlockWaves, D = NH * kD, C = D / kWave;
+  __shared__ BlockLds<REP, Q8, NH> sm;
+  const int wi = (int)(threadIdx.x / kWave), lane = (int)(threadIdx.x % kWave);
+  const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv), s = (int)(blockIdx.x / (unsigned)a.n_kv);
+  int L = a.kv_len[s];
+  L = L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : max(L, 0);
+  const PrefixRows pr = prefix_rows(x, s, a.n_heads);
+  const int np = (L + kPage - 1) / kPage, per = (np + NW - 1) / NW, i0 = min(np, wi * per), i1 = min(np, i0 + per);
+  if (i0 < i1) {
+    PieceLoads<REP, NH> pl;
+    piece_loads<REP, false, false, Q8, NH>(a, s, kvh, i0, pl);
+    const int e = i0 + lane;  // the wave's pages are fewer than the window's 64
+    if (e < a.bt_stride && e < pr.pages) pl.btv = a.bt[(size_t)pr.first * a.bt_stride + e];
+    block_piece<REP, Q8, NH>(a, sm, wi, s, kvh, pl, 0, i0, i1, L);
+  }
+  __syncthreads();
+  const int nw = np > 0 ? (np + per - 1) / per : 0;  // waves that left rows
+  for (int h = wi; h < REP; h += NW) {  // wave-uniform
+    float M, Ls, A[C];
+    block_merge<REP, Q8, NH>(sm, nw, h, M, Ls, A);
+    const size_t row = ((size_t)s * a.n_heads + (size_t)kvh * REP + h) * D;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const size_t i = row + c * kWave + lane;
+      a.out[i] = gated(a, i, Ls > 0.0f ? A[c] / Ls : 0.0f);
     }
   }
 }
@@ -503,6 +554,16 @@ void launch_own_rep(const DecodeArgs& a, const OwnArgs& x, int rep, unsigned blo
   }
 }
 
+template <bool Q8, int NH>
+void launch_block_rep(const DecodeArgs& a, const VarArgs<kPrefix>& x, int rep, unsigned blocks, hipStream_t st) {
+  switch (rep) {
+    case 1: prefix_block_kernel<1, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
+    case 2: prefix_block_kernel<2, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
+    case 4: prefix_block_kernel<4, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
+    default: prefix_block_kernel<8, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
+  }
+}
+
 template <bool Q8>
 void launch_prefix_mfma(const PrefixArgs& a, int d, int tile_rows, unsigned blocks, hipStream_t st) {
   if (d == 256)
@@ -526,6 +587,7 @@ void launch_prefix_tile(const PrefixArgs& a, int d, int64_t items, hipStream_t s
 // ---------------------------------------------------------------------------
 // The host's view of a call.
 struct PrefixPlan {
+  bool direct = false;    // one launch: every sequence reads the shared pages itself
   VarPlan own;            // the tile kernel over the sequences' own pages
   int shares = 0;         // own kernel: shares of a sequence at most (0: the tile kernel)
   int share_pages = 0;
@@ -568,6 +630,15 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   if (at < n_seq) most = all;
   own_pages += (n_seq - at) * all;
   const size_t row = ((size_t)d + 2) * sizeof(float);
+  const int64_t bytes = all * kPage * 2 * d * n_seq * c->n_kv_heads *
+                        (c->dtype == LNSKV_DTYPE_F32 ? 4 : c->dtype == LNSKV_DTYPE_F16 ? 2 : 1);
+  const bool wide_f32 = c->dtype == LNSKV_DTYPE_F32 && d > 64;
+  p->direct = schedule_setting() == kScheduleAuto && all <= (wide_f32 ? kDirectPages / 2 : kDirectPages) &&
+              bytes <= kDirectBytes;
+  if (p->direct) {
+    p->own.split = (int)all * kPage;
+    return LNSKV_OK;
+  }
   if (var_mfma(c)) {
     // shares of at most kSharePages pages, fewer where that leaves compute units idle
     const int64_t units = own_pages * c->n_kv_heads;
@@ -650,9 +721,21 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
   o.shares = p.shares;
   o.share_pages = p.share_pages;
   o.prefix.n_groups = p.n_groups;
-  o.prefix.split_pages = p.split_pages;
+  o.prefix.split_pages = p.direct ? 0 : p.split_pages;
   std::copy(p.g, p.g + p.n_groups, o.prefix.g);
-  if (p.n_groups > 0) {
+  if (p.direct && var_mfma(c)) {
+    const unsigned blocks = (unsigned)(n_seq * a.n_kv);
+    const int rep = n_heads / a.n_kv;
+    if (c->dtype == LNSKV_DTYPE_Q8A) {
+      if (d == 256) launch_block_rep<true, 2>(a, o.prefix, rep, blocks, st);
+      else launch_block_rep<true, 1>(a, o.prefix, rep, blocks, st);
+    } else {
+      if (d == 256) launch_block_rep<false, 2>(a, o.prefix, rep, blocks, st);
+      else launch_block_rep<false, 1>(a, o.prefix, rep, blocks, st);
+    }
+    return hip_check("decode kernel launch");
+  }
+  if (p.n_groups > 0 && !p.direct) {
     PrefixArgs x{};
     x.pf.k_pages = a.k_pages;
     x.pf.v_pages = a.v_pages;

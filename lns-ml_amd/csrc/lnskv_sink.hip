@@ -39,7 +39,11 @@ void sink_block_kernel(DecodeArgs a, VarArgs<kSink> x) {
   const SinkSpan sp = sink_span(x, L);
   const int np = L > 0 ? (L - 1) / kPage + 1 - sp.gap : 0;
   const int per = (np + NW - 1) / NW, i0 = min(np, wi * per), i1 = min(np, i0 + per);
-  if (i0 < i1) block_piece<REP, Q8, NH, kSink>(a, sm, wi, s, kvh, 0, i0, i1, L, sp);
+  if (i0 < i1) {
+    PieceLoads<REP, NH> pl;
+    piece_loads<REP, false, false, Q8, NH, kSink>(a, s, kvh, i0, pl, sp);
+    block_piece<REP, Q8, NH, kSink>(a, sm, wi, s, kvh, pl, 0, i0, i1, L, sp);
+  }
   __syncthreads();
   const int nw = np > 0 ? (np + per - 1) / per : 0;  // waves that left rows
   for (int h = wi; h < REP; h += NW) {  // wave-uniform

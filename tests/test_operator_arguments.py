@@ -103,7 +103,7 @@ def test_sink_decode_refuses(kw, rc, text):
     (dict(groups=((0, 1, -1),)), INV, "group 0"), (dict(groups=((1, 1, 32), (0, 1, 32))), INV, "group 1"),
     (dict(groups=((0, 2, 32), (1, 1, 32))), INV, "group 1"), (dict(groups=((1, 2**31 - 1, 32),)), INV, "group 0"),
     (dict(groups=None, n_groups=1), INV, "non-null"), (dict(n_groups=-1), INV, "n_groups"),
-    (dict(groups=[(i, 1, 32) for i in range(129)], n_seq=200), INV, "n_groups"), (dict(ws_bytes=4096), WS, "needed"),
+    (dict(groups=[(i, 1, 32) for i in range(129)], n_seq=200), INV, "n_groups"), (dict(max_len=4096, ws_bytes=4096), WS, "needed"),
 ])
 def test_prefix_decode_refuses(kw, rc, text):
     got, msg = prefix(**kw)
@@ -117,7 +117,7 @@ def test_prefix_decode_of_large_q8a_pools():
     assert got == UNS and "2 GiB" in msg
     for ok in (pages(_lib.DTYPE_Q8A, 128, kv=8, n=(1 << 22) - 1), pages(_lib.DTYPE_F16, 128, kv=8, n=1 << 22),
                pages(_lib.DTYPE_Q8A, 64, kv=8, n=1 << 22)):
-        got, msg = prefix(c=ok, n_heads=8, ws_bytes=16)  # further checks come after
+        got, msg = prefix(c=ok, n_heads=8, max_len=4096, ws_bytes=16)  # further checks come after
         assert got == WS and "needed" in msg
 
 
@@ -169,6 +169,8 @@ def test_workspace_queries():
     assert lib.lnskv_prefix_decode_workspace_size(C.byref(c), None, 0, 2, 8, 40, C.byref(out)) == 0
     assert out.value == 0  # nothing shared, one partition
     assert lib.lnskv_prefix_decode_workspace_size(C.byref(c), g, 1, 2, 8, 64, C.byref(out)) == 0
+    assert out.value == 0  # short: one launch
+    assert lib.lnskv_prefix_decode_workspace_size(C.byref(c), g, 1, 2, 8, 4096, C.byref(out)) == 0
     assert out.value >= 4096 + 2 * 8 * (64 + 2) * 4  # a row per query head
 
 
