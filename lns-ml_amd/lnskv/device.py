@@ -28,25 +28,7 @@ def _stream(device: torch.device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-class _on:
-    """Makes a device current for a call (streams and workspaces are per device) and
-    yields its current stream; does nothing else where it is current already."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        now = torch._C._cuda_getDevice()
-        self.before = now if now != self.index else None
-        if self.before is not None:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+_TABLE_TYPES = (torch.int32, torch.uint32)
 
 
 def _need(t: torch.Tensor, name: str, dtype, numel: int, device) -> None:
@@ -117,10 +99,22 @@ class PagedKV:
 
     def _any_tables(self, tables: torch.Tensor) -> int:
         """Block tables of any number of rows; returns their stride."""
-        if tables.dim() != 2 or tables.dtype not in (torch.int32, torch.uint32):
+        shape = tables.shape
+        if len(shape) != 2 or tables.dtype not in _TABLE_TYPES:
             raise ValueError("block tables must be 2-D, int32 or uint32")
-        _need(tables, "block_tables", tables.dtype, tables.numel(), self.device)
-        return int(tables.shape[1])
+        if tables.device != self.device or not tables.is_contiguous():
+            raise ValueError(f"block_tables must be contiguous and on {self.device}, got {tables.device}")
+        return shape[1]
+
+    def _run(self, fn, *args) -> None:
+        """fn(*args, stream) on the pools' device (streams and workspaces are per device)
+        and its current stream."""
+        index = self.device.index
+        if torch._C._cuda_getDevice() == index:
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+        else:
+            with torch.cuda.device(index):
+                check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
     def _variant_common(self, q, tables, kv_len, n_heads, gate, workspace, out):
         n_seq, stride = self._decode_common(q, tables, kv_len, None, n_heads)
@@ -289,7 +283,7 @@ class PagedKV:
         and V of every token into the slots of tok_pos; q [n_tok][n_heads][d], when
         given, turned the same way into q_out (q itself, or None: a new tensor),
         which is returned."""
-        n_tok = int(tok_seq.numel())
+        n_tok = tok_seq.numel()
         dev = self.device
         _need(k_new, "k_new", torch.float32, n_tok * self.row_elems, dev)
         _need(v_new, "v_new", torch.float32, n_tok * self.row_elems, dev)
@@ -310,16 +304,14 @@ class PagedKV:
             _need(q_out, "q_out", torch.float32, q.numel(), dev)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        with _on(dev) as stream:
-            check(lib().lnskv_mrope_append(self._c, rope._c, rope._sections, rope.n_axes, rope.interleaved, _address(q),
-                                           _address(q_out), n_heads, k_new.data_ptr(), v_new.data_ptr(), axis_pos.data_ptr(),
-                                           tok_seq.data_ptr(), tok_pos.data_ptr(), n_tok, tables.data_ptr(), stride,
-                                           int(tables.shape[0]), stream))
+        self._run(lib().lnskv_mrope_append, self._c, rope._c, rope._sections, rope.n_axes, rope.interleaved, _address(q),
+                  _address(q_out), n_heads, k_new.data_ptr(), v_new.data_ptr(), axis_pos.data_ptr(), tok_seq.data_ptr(),
+                  tok_pos.data_ptr(), n_tok, tables.data_ptr(), stride, tables.shape[0])
         return q_out
 
     def sink_workspace_size(self, n_seq: int, n_heads: int, max_kv_len: int, window: int, n_sink: int) -> int:
         out = C.c_size_t()
-        with _on(self.device):
+        with torch.cuda.device(self.device):
             check(lib().lnskv_sink_decode_workspace_size(self._c, n_seq, n_heads, max_kv_len, window, n_sink,
                                                          C.byref(out)))
         return out.value
@@ -329,10 +321,8 @@ class PagedKV:
         """lnskv_sink_decode: every sequence attends its first n_sink tokens and its
         last `window` (0: all of them)."""
         n_seq, stride, out, ws_bytes = self._variant_common(q, tables, kv_len, n_heads, gate, workspace, out)
-        with _on(self.device) as stream:
-            check(lib().lnskv_sink_decode(self._c, _address(q), out.data_ptr(), _address(gate), tables.data_ptr(), stride, kv_len.data_ptr(),
-                                          n_seq, n_heads, max_kv_len, window, n_sink, scale, _address(workspace),
-                                          ws_bytes, stream))
+        self._run(lib().lnskv_sink_decode, self._c, q.data_ptr(), out.data_ptr(), _address(gate), tables.data_ptr(), stride,
+                  kv_len.data_ptr(), n_seq, n_heads, max_kv_len, window, n_sink, scale, _address(workspace), ws_bytes)
         return out
 
     def sink_prefill_workspace_size(self, n_chunks: int, n_tok: int, stride: int, window: int, n_sink: int,
@@ -359,15 +349,14 @@ class PagedKV:
         if workspace is not None:
             _need(workspace, "workspace", workspace.dtype, workspace.numel(), self.device)
             ws_bytes = workspace.numel() * workspace.element_size()
-        with _on(self.device) as stream:
-            check(lib().lnskv_sink_prefill_attention(self._c, _address(q), out.data_ptr(), chunks.data_ptr(), int(chunks.shape[0]),
-                                                     n_tok, tables.data_ptr(), stride, int(tables.shape[0]), window,
-                                                     n_sink, n_heads, scale, _address(workspace), ws_bytes, stream))
+        self._run(lib().lnskv_sink_prefill_attention, self._c, q.data_ptr(), out.data_ptr(), chunks.data_ptr(),
+                  chunks.shape[0], n_tok, tables.data_ptr(), stride, tables.shape[0], window, n_sink, n_heads, scale,
+                  _address(workspace), ws_bytes)
         return out
 
     def prefix_workspace_size(self, groups: "PrefixGroups", n_seq: int, n_heads: int, max_kv_len: int) -> int:
         out = C.c_size_t()
-        with _on(self.device):
+        with torch.cuda.device(self.device):
             check(lib().lnskv_prefix_decode_workspace_size(self._c, groups._p, groups.n, n_seq, n_heads, max_kv_len,
                                                            C.byref(out)))
         return out.value
@@ -377,10 +366,8 @@ class PagedKV:
         """lnskv_prefix_decode: decode in which the sequences of each group read
         their shared leading pages once for all (from the group's first row)."""
         n_seq, stride, out, ws_bytes = self._variant_common(q, tables, kv_len, n_heads, gate, workspace, out)
-        with _on(self.device) as stream:
-            check(lib().lnskv_prefix_decode(self._c, _address(q), out.data_ptr(), _address(gate), tables.data_ptr(), stride,
-                                            kv_len.data_ptr(), groups._p, groups.n, n_seq, n_heads, max_kv_len, scale,
-                                            _address(workspace), ws_bytes, stream))
+        self._run(lib().lnskv_prefix_decode, self._c, q.data_ptr(), out.data_ptr(), _address(gate), tables.data_ptr(), stride,
+                  kv_len.data_ptr(), groups._p, groups.n, n_seq, n_heads, max_kv_len, scale, _address(workspace), ws_bytes)
         return out
 
     def attention_paged(self, q, k_in, v_in, block_table, pos: int, n_heads: int, p_start: int = 0,
