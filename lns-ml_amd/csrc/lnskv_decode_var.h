@@ -23,12 +23,16 @@ struct VarPlan {
   size_t ws_bytes = 0;
 };
 
-// Tokens of a sequence up to which one block takes them all, and the fewest that a
-// partition has otherwise.  Us: 7 sequences x 8 kv heads of 240 tokens, Q8A, 64-wide: one
-// block 7.7, partitions of 64 10.7, of 128 10.2 (a second launch merges); 24 x 4 of 1021,
-// f32: of 64 16.6, 128 15.3, 192 17.5, 256 15.8, 512 19.5; 3 x 4 of 3700, Q8A: 12.3, 11.0,
-// 10.9, 11.6, 16.2.
+// Tokens of a sequence up to which one block takes them all (kOnePartitionFull where the
+// (sequence, kv head) pairs are about as many as the compute units), and the fewest that a
+// partition has otherwise.  Us, one block | partitions and a second launch that merges
+// them: 7 sequences x 8 kv heads of 240 tokens, Q8A, 64-wide 7.7 | 10.2; 48 x 4 of 700, f32
+// 16.8 | 21.5, f32 256-wide 54.7 | 84.0, f16 18.7 | 19.2, of 960 23.3 | 21.8; but 12 x 4 of
+// 440, f32 12.2 | 9.6, of 700 15.9 | 11.5.  Partitions of 64 | 128 | 192 | 256 | 512 tokens:
+// 24 x 4 of 1021, f32 16.6 | 15.3 | 17.5 | 15.8 | 19.5; 3 x 4 of 3700, Q8A 12.3 | 11.0 |
+// 10.9 | 11.6 | 16.2.
 constexpr int kOnePartition = 256;
+constexpr int kOnePartitionFull = 768;
 constexpr int kLeastPartition = 128;
 
 inline bool var_mfma(const lnskv_pages* c) {
@@ -39,8 +43,10 @@ inline bool var_mfma(const lnskv_pages* c) {
 // where those are few (a block's four waves share it and no merge is launched).
 inline int plan_tiles(const lnskv_pages* c, int n_seq, int n_heads, int64_t pages, VarPlan* p) {
   const int64_t tokens = std::max<int64_t>(pages, 1) * kPage;
-  p->split = tokens <= kOnePartition ? (int)tokens
-                                     : std::max(kLeastPartition, choose_split(n_seq, (int)c->n_kv_heads, (int)std::min<int64_t>(tokens, INT32_MAX / 2)));
+  const int64_t one = (int64_t)n_seq * c->n_kv_heads >= 192 ? kOnePartitionFull : kOnePartition;
+  p->split = (int)tokens;
+  if (tokens > one)
+    p->split = std::max(kLeastPartition, choose_split(n_seq, (int)c->n_kv_heads, (int)std::min<int64_t>(tokens, INT32_MAX / 2)));
   const int64_t parts = (tokens + p->split - 1) / p->split;
   if (parts > 65535)
     return fail(LNSKV_ERR_INVALID, "%lld tokens a sequence need more than 65535 partitions", (long long)tokens);

@@ -79,6 +79,7 @@ def test_decode_of_many_sequences(dtype):
     lens = [int(x) for x in rng.integers(1, 300, 150)]
     assert decode_case(dtype, 128, 2, 4, lens, 40, 4, seed=8) < A.TOL
     assert decode_case(dtype, 128, 2, 4, [4 * L for L in lens[:100]], 800, 4, seed=9) < A.TOL
+    assert decode_case(dtype, 64, 2, 4, [4 * L for L in lens[:100]], 700, 33, seed=9) < A.TOL
 
 
 @pytest.mark.parametrize("dtype", [DTYPE_F16, DTYPE_Q8A])
