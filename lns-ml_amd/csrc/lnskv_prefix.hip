@@ -14,8 +14,8 @@
 //    a sequence with one share merges the prefix's rows and writes its output.
 // 3. join kernel, where sequences may have several shares: their rows and the
 //    prefix's into the output.
-// Short sequences take one launch instead, in which each reads its group's pages
-// itself (block kernel, or the tile kernel).
+// Small calls take one launch instead, in which each sequence reads its group's pages
+// itself (block kernel, or the tile kernel and its merge).
 #include "lnskv_decode_block.h"
 #include "lnskv_decode_var.h"
 #include "lnskv_prefill.h"
@@ -42,17 +42,22 @@ constexpr int kWidePages = 48;
 constexpr int kSharePages = 64;
 constexpr int kShareMin = 8;
 constexpr int kShareWhole = 32;
-// Sequences of at most kDirectPages pages (half of that with 128- and 256-wide f32 heads,
-// whose f32 products take longest) and kDirectBytes of K and V, shared pages counted
-// every time, are decoded in one launch in which each reads its group's pages itself, from
-// L2 mostly.  Us, one launch | prefix and own pages apart, sequences x kv heads of pages:
-// f16 128-wide 4 x 8 of 13 7.3 | 13.8, 16 x 8 of 57 13.3 | 19.2, 64 x 8 of 57 (228 MB) 22.3
-// | 26.4, 128 x 8 of 57 (456 MB) 42.6 | 39.9, 16 x 8 of 107 20.8 | 21.2, 64 x 8 of 107 37 |
-// 28.5; Q8A 128 x 8 of 57 (228 MB) 39.4 | 36.7, 256-wide 64 x 4 of 26 17.4 | 26.6; f32
-// 64-wide 2 x 4 of 21 8.8 | 12.6, 128-wide 64 x 8 of 13 (104 MB) 17.0 | 22.2, of 26 (208 MB)
-// 26.8 | 23.2, 4 x 8 of 57 23.2 | 20.7.
+// Small calls take one launch in which every sequence reads its group's pages itself, from
+// L2 mostly: on the matrix cores sequences of at most kDirectPages pages, kDirectBytes of K
+// and V in all, shared pages counted every time.  Us, one launch | prefix and own pages
+// apart, sequences x kv heads of pages: f16 128-wide 4 x 8 of 13 7.3 | 13.8, 16 x 8 of 57
+// 13.3 | 19.2, 64 x 8 of 57 (228 MB) 22.3 | 26.4, 128 x 8 of 57 (456 MB) 42.6 | 39.9, 16 x 8
+// of 107 20.8 | 21.2, 64 x 8 of 107 37 | 28.5; Q8A 128 x 8 of 57 (228 MB) 39.4 | 36.7,
+// 256-wide 64 x 4 of 26 17.4 | 26.6.
+// On the tile kernel kDirectUnits x (7 + heads per kv head) pages of 64 elements (a wave's
+// products cost the same for one head and for 16, so what the prefix kernel saves by tiles
+// of 16 rows falls with the heads): f32, 8 heads on one, 2 x 4 of 588 14 | 56, 6 x 4 of 588
+// 24 | 41, 20 x 4 of 194 25.9 | 25.6, 60 x 4 of 88 32 | 27, 128-wide 60 x 4 of 32 19 | 25, 20
+// x 4 of 194 47 | 36; 2 heads, 128-wide 6 x 8 of 88 16 | 22, 20 x 8 of 32 19.9 | 17.6; Q8A, 1
+// head 6 x 8 of 194 15.2 | 15.7, 60 x 8 of 32 17.7 | 15.1.
 constexpr int kDirectPages = 64;
 constexpr int64_t kDirectBytes = (int64_t)192 << 20;
+constexpr int64_t kDirectUnits = 1024;
 
 struct PrefixArgs {
   PrefillArgs pf;  // the pools, for the prefill kernel's page pipeline
@@ -630,14 +635,16 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   if (at < n_seq) most = all;
   own_pages += (n_seq - at) * all;
   const size_t row = ((size_t)d + 2) * sizeof(float);
-  const int64_t bytes = all * kPage * 2 * d * n_seq * c->n_kv_heads *
-                        (c->dtype == LNSKV_DTYPE_F32 ? 4 : c->dtype == LNSKV_DTYPE_F16 ? 2 : 1);
-  const bool wide_f32 = c->dtype == LNSKV_DTYPE_F32 && d > 64;
-  p->direct = schedule_setting() == kScheduleAuto && all <= (wide_f32 ? kDirectPages / 2 : kDirectPages) &&
-              bytes <= kDirectBytes;
-  if (p->direct) {
-    p->own.split = (int)all * kPage;
-    return LNSKV_OK;
+  if (schedule_setting() == kScheduleAuto) {  // one launch for all pages
+    const int64_t units = all * n_seq * c->n_kv_heads;
+    const int64_t bytes = units * kPage * 2 * d * (c->dtype == LNSKV_DTYPE_F16 ? 2 : 1);
+    if (var_mfma(c) ? all <= kDirectPages && bytes <= kDirectBytes : units * (d / 64) <= kDirectUnits * (7 + rep)) {
+      p->direct = true;
+      if (var_mfma(c)) return LNSKV_OK;
+      if (int rc = plan_tiles(c, n_seq, n_heads, all, &p->own)) return rc;
+      p->ws_bytes = p->own.ws_bytes;
+      return LNSKV_OK;
+    }
   }
   if (var_mfma(c)) {
     // shares of at most kSharePages pages, fewer where that leaves compute units idle
