@@ -1,7 +1,7 @@
-// Decode attention on pages that the f16 matrix products do not take (f32 pages, and
-// 64-wide heads of every page type), for the decode variants: both products as
-// v_mfma_f32_16x16x4_f32, one wave per page, 16 query rows, no LDS and no exchange
-// between lanes but for the maxima.
+// Decode attention on f32 pages and on 64-wide heads of every page type, for the decode
+// variants: a wave per page and 16 query rows, no LDS and no exchange between lanes but
+// for the maxima.  f32 pages in v_mfma_f32_16x16x4_f32; f16 and Q8A pages (codes are exact
+// in f16) in f16 products with q and the weights as hi and lo parts.
 //
 // Lane (g, n) = (lane / 16, lane % 16).  A contraction may take its index in any
 // order, as long as both operands take the same, so each operand is what a lane
@@ -14,15 +14,17 @@
 //   for row n the lane already holds.  It loads elements 64 c + 4n + e of that
 //   token (a row of V per 16 lanes); product (ii, c, e) gives output columns
 //   64 c + 4n + e of rows 4g + i.  A masked token's V is its own lanes' to clear.
-// A page takes D / 2 products of 32 cycles whatever its type and head count, against
-// which HBM delivers f32 and f16 pages later; Q8A pages of 64-wide heads at about the
-// same rate.  24 sequences x 4 kv heads of 8, window 1000 + 21, f32, 64-wide: 13.2 us and
-// 4.0 for the merge (44 MB take 9.2 at a large copy's rate); the generic decode kernel's
-// vector code took 21.8.  Three sequences of 3700 Q8A tokens 11 us (34: its sums across
-// rows at the end of every block).
+// f16 products take the same elements eight at a time (scores, over 32 of them) and the
+// four tokens of a lane at once (P.V).
+// A page takes D / 2 f32 products of 32 cycles, or 4 + 8 f16 products of 16, whatever the
+// head count: bound by HBM, or by start-up and the merge where partitions are short.  24
+// sequences x 4 kv heads of 8, window 1000 + 21, f32, 64-wide: 13.2 us and 4.0 for the
+// merge (44 MB take 9.2 at a large copy's rate); the generic decode kernel's vector code
+// took 21.8.  48 x 4 of 3000, f16, 64-wide: 39 us (147 MB, 31).  Sixty sequences of 9400
+// tokens behind 9000 shared ones, f16: 44 us with f16 products, 78 with f32 ones.
 #pragma once
 
-#include "lnskv_device.h"
+#include "lnskv_mfma.h"
 
 namespace lnskv {
 namespace {
@@ -44,18 +46,24 @@ struct TilePage {
   float ks, vs;  // Q8A: of token 4g + n % 4
 };
 
+// f16 and Q8A pages (64-wide heads): f16 products, q and the weights as pairs of f16.
+template <int DT>
+constexpr bool kTileHalf = DT != LNSKV_DTYPE_F32;
+
 template <int DT, int D>
 struct TileState {
-  float q[D / 4];
-  float4v acc[D / 16];  // [4 c + e][i]: O[row 4g + i][64 c + 4n + e]
+  float q[kTileHalf<DT> ? 1 : D / 4];
+  half8 qh[kTileHalf<DT> ? 2 : 1], ql[kTileHalf<DT> ? 2 : 1];  // q / 2^E, hi and lo
+  float qexp;           // 2^E
+  float4v acc[D / 16];  // [4 c + e][i]: O[row 4g + i][64 c + 4n + e] (Q8A: over vnorm)
   float m, l;           // of row n (l: over this lane's tokens)
+  float vnorm, vinv;    // Q8A: a power of two that follows the largest V scale, and 1 over it
 };
 
 template <int DT>
 __device__ __forceinline__ float tile_elem(const uint32_t* w, int e) {
-  if constexpr (DT == LNSKV_DTYPE_F32) return __builtin_bit_cast(float, w[e]);
-  else if constexpr (DT == LNSKV_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e / 2] >> (16 * (e & 1))));
-  else return (float)(int8_t)(w[e / 4] >> (8 * (e & 3)));
+  static_assert(!kTileHalf<DT>);
+  return __builtin_bit_cast(float, w[e]);
 }
 
 template <int N>
@@ -96,18 +104,89 @@ __device__ __forceinline__ void tile_load(const Args& a, uint32_t phys, int kvh,
 template <int DT, int D>
 __device__ __forceinline__ void tile_init(TileState<DT, D>& st, const float* q, float scale, int g) {
   using G = TileGeo<DT, D>;
+  static_assert(!kTileHalf<DT> || D == 64, "two f16 products per page");
+  float x[D / 4];
 #pragma unroll
   for (int j = 0; j < G::KL; ++j)
 #pragma unroll
-    for (int x = 0; x < G::E / 4; ++x) {
-      const float4v w = *reinterpret_cast<const float4v*>(q + 4 * G::E * j + G::E * g + 4 * x);
+    for (int y = 0; y < G::E / 4; ++y) {
+      const float4v w = *reinterpret_cast<const float4v*>(q + 4 * G::E * j + G::E * g + 4 * y);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st.q[G::E * j + 4 * x + e] = w[e] * scale;
+      for (int e = 0; e < 4; ++e) x[G::E * j + 4 * y + e] = w[e] * scale;
     }
+  if constexpr (kTileHalf<DT>) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    amax = max_xor16(max_xor32(amax));
+    int E = 0;
+    if (amax > 0.0f && amax < INFINITY) (void)frexpf(amax, &E);
+    const float inv = ldexpf(1.0f, -E);
+    st.qexp = ldexpf(1.0f, E);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float y = x[i] * inv;
+      const _Float16 hi = (_Float16)y;
+      st.qh[i / 8][i % 8] = hi;
+      st.ql[i / 8][i % 8] = (_Float16)(y - (float)hi);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) st.q[i] = x[i];
+  }
 #pragma unroll
   for (int b = 0; b < D / 16; ++b) st.acc[b] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   st.m = kMInit;
-  st.l = 0.0f;
+  st.l = st.vnorm = st.vinv = 0.0f;
+}
+
+// Elements 4 n .. of rows 4g + i, columns 64 c + 4n ..
+template <int DT, int D>
+__device__ __forceinline__ float4v tile_out(const TileState<DT, D>& st, int c, int i) {
+  const float4v o = {st.acc[4 * c][i], st.acc[4 * c + 1][i], st.acc[4 * c + 2][i], st.acc[4 * c + 3][i]};
+  return DT == LNSKV_DTYPE_Q8A ? o * st.vnorm : o;
+}
+
+// The products of a page of f16 or Q8A: scores of tokens 4g + ii of row n (Q8A: without
+// the scales), and P.V.
+template <int DT, int D>
+__device__ __forceinline__ float4v tile_scores_half(const TileState<DT, D>& st, const TilePage<DT, D>& pg) {
+  float4v s = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = s;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    half8 k;
+    if constexpr (DT == LNSKV_DTYPE_F16) k = __builtin_bit_cast(half8, u32x4{pg.k[j][0], pg.k[j][1], pg.k[j][2], pg.k[j][3]});
+    else k = i8x8_to_f16(uint2v{pg.k[0][2 * j], pg.k[0][2 * j + 1]});
+    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, st.qh[j], s, 0, 0, 0);
+    s2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, st.ql[j], s2, 0, 0, 0);
+  }
+  return (s + s2) * st.qexp;
+}
+template <int DT, int D>
+__device__ __forceinline__ void tile_pv_half(TileState<DT, D>& st, const TilePage<DT, D>& pg, const float (&p)[4]) {
+  half4 ph, pl, v[4];  // v[ii][e]: token 4g + ii, element 4n + e
+#pragma unroll
+  for (int ii = 0; ii < 4; ++ii) {
+    ph[ii] = (_Float16)p[ii];
+    pl[ii] = (_Float16)(p[ii] - (float)ph[ii]);
+  }
+#pragma unroll
+  for (int ii = 0; ii < 4; ii += 2) {
+    if constexpr (DT == LNSKV_DTYPE_F16) {
+      v[ii] = __builtin_bit_cast(half4, uint2v{pg.v[ii][0][0], pg.v[ii][0][1]});
+      v[ii + 1] = __builtin_bit_cast(half4, uint2v{pg.v[ii + 1][0][0], pg.v[ii + 1][0][1]});
+    } else {
+      const half8 x = i8x8_to_f16(uint2v{pg.v[ii][0][0], pg.v[ii + 1][0][0]});
+      v[ii] = half4{x[0], x[1], x[2], x[3]};
+      v[ii + 1] = half4{x[4], x[5], x[6], x[7]};
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const half4 b = {v[0][e], v[1][e], v[2][e], v[3][e]};
+    st.acc[e] = __builtin_amdgcn_mfma_f32_16x16x16f16(ph, b, st.acc[e], 0, 0, 0);
+    st.acc[e] = __builtin_amdgcn_mfma_f32_16x16x16f16(pl, b, st.acc[e], 0, 0, 0);
+  }
 }
 
 // One page through the online softmax.  full: every row attends every token.
@@ -117,15 +196,20 @@ template <int DT, int D, class Sees, class Any>
 __device__ __forceinline__ void tile_consume(TileState<DT, D>& st, TilePage<DT, D>& pg, bool full, int g, Sees sees,
                                              Any any) {
   using G = TileGeo<DT, D>;
-  float4v s = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = s;
+  float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (kTileHalf<DT>) {
+    s = tile_scores_half<DT, D>(st, pg);
+  } else {
+    float4v s2 = s;
 #pragma unroll
-  for (int j = 0; j < G::KL; ++j)
+    for (int j = 0; j < G::KL; ++j)
 #pragma unroll
-    for (int e = 0; e < G::E; e += 2) {
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_elem<DT>(pg.k[j], e), st.q[G::E * j + e], s, 0, 0, 0);
-      s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_elem<DT>(pg.k[j], e + 1), st.q[G::E * j + e + 1], s2, 0, 0, 0);
-    }
-  s += s2;
+      for (int e = 0; e < G::E; e += 2) {
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_elem<DT>(pg.k[j], e), st.q[G::E * j + e], s, 0, 0, 0);
+        s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(tile_elem<DT>(pg.k[j], e + 1), st.q[G::E * j + e + 1], s2, 0, 0, 0);
+      }
+    s += s2;
+  }
   float vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
   if constexpr (DT == LNSKV_DTYPE_Q8A) {
     s[0] *= dpp_mov<0x00>(pg.ks), s[1] *= dpp_mov<0x55>(pg.ks), s[2] *= dpp_mov<0xAA>(pg.ks), s[3] *= dpp_mov<0xFF>(pg.ks);
@@ -163,15 +247,38 @@ __device__ __forceinline__ void tile_consume(TileState<DT, D>& st, TilePage<DT, 
 #pragma unroll
   for (int ii = 0; ii < 4; ++ii) p[ii] = fast_exp2(s[ii] - st.m);
   st.l += (p[0] + p[1]) + (p[2] + p[3]);
+  if constexpr (DT == LNSKV_DTYPE_Q8A) {  // f16 weights: over a power of two near the largest scale
+    const float vmax = max_xor16(max_xor32(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]))));
+    if ((vmax > st.vnorm || vmax * 16.0f < st.vnorm) && vmax > 0.0f) {  // wave-uniform
+      int e = 0;
+      (void)frexpf(vmax, &e);
+      if (st.vnorm > 0.0f) {
+        const float r = st.vnorm * ldexpf(1.0f, -e);
 #pragma unroll
-  for (int ii = 0; ii < 4; ++ii) {
-    if constexpr (DT == LNSKV_DTYPE_Q8A) p[ii] *= vs[ii];
+        for (int b = 0; b < D / 16; ++b) st.acc[b] *= r;
+      }
+      st.vnorm = ldexpf(1.0f, e);
+      st.vinv = ldexpf(1.0f, -e);
+    }
 #pragma unroll
-    for (int c = 0; c < G::C; ++c)
+    for (int ii = 0; ii < 4; ++ii) {
+      p[ii] *= vs[ii] * st.vinv;
+      // one rounded product for both parts: contracted into the conversions, a product
+      // beside a tie of f16 rounds to one hi part and is subtracted from another
+      asm("" : "+v"(p[ii]));
+    }
+  }
+  if constexpr (kTileHalf<DT>) {
+    tile_pv_half<DT, D>(st, pg, p);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        st.acc[4 * c + e] =
-            __builtin_amdgcn_mfma_f32_16x16x4f32(p[ii], tile_elem<DT>(pg.v[ii][c], e), st.acc[4 * c + e], 0, 0, 0);
+    for (int ii = 0; ii < 4; ++ii)
+#pragma unroll
+      for (int c = 0; c < G::C; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          st.acc[4 * c + e] =
+              __builtin_amdgcn_mfma_f32_16x16x4f32(p[ii], tile_elem<DT>(pg.v[ii][c], e), st.acc[4 * c + e], 0, 0, 0);
   }
 }
 
@@ -254,7 +361,7 @@ __global__ __launch_bounds__(kBlock) void decode_tile_kernel(DecodeArgs a, VarAr
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
         *reinterpret_cast<float4v*>(&sm.acc[wave][4 * g + i][64 * c + 4 * n]) =
-            float4v{st.acc[4 * c][i], st.acc[4 * c + 1][i], st.acc[4 * c + 2][i], st.acc[4 * c + 3][i]};
+            tile_out<DT, D>(st, c, i);
     }
   __syncthreads();
   finish_block<REP, D, VAR>(a, sm, w, s, kvh, part, x);

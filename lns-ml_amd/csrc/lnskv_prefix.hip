@@ -53,8 +53,8 @@ constexpr int kShareWhole = 32;
 // products cost the same for one head and for 16, so what the prefix kernel saves by tiles
 // of 16 rows falls with the heads): f32, 8 heads on one, 2 x 4 of 588 14 | 56, 6 x 4 of 588
 // 24 | 41, 20 x 4 of 194 25.9 | 25.6, 60 x 4 of 88 32 | 27, 128-wide 60 x 4 of 32 19 | 25, 20
-// x 4 of 194 47 | 36; 2 heads, 128-wide 6 x 8 of 88 16 | 22, 20 x 8 of 32 19.9 | 17.6; Q8A, 1
-// head 6 x 8 of 194 15.2 | 15.7, 60 x 8 of 32 17.7 | 15.1.
+// x 4 of 194 47 | 36; 2 heads, 128-wide 6 x 8 of 88 16 | 22, 20 x 8 of 32 19.9 | 17.6; f16,
+// 64-wide, 8 heads 6 x 4 of 588 19 | 36, 1 head 6 x 8 of 88 9.6 | 13.8.
 constexpr int kDirectPages = 64;
 constexpr int64_t kDirectBytes = (int64_t)192 << 20;
 constexpr int64_t kDirectUnits = 1024;
@@ -127,7 +127,7 @@ __device__ __forceinline__ int row_tokens(const PrefixArgs& a, int s, int pages)
 }
 
 // ---------------------------------------------------------------------------
-// f32 pages, and 64-wide heads on every page type, in f32 (lnskv_decode_tile.h): a
+// f32 pages, and 64-wide heads on every page type (lnskv_decode_tile.h): a
 // wave per item of 16 rows and one split.  The waves of a block take the tiles of
 // one split, or consecutive splits of few rows, and share nothing but the cache.
 // Bound by the products (v_mfma_f32_16x16x4_f32, 32 cycles) once groups are large: 109
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kBlock) void prefix_tile_kernel(PrefixArgs a) {
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
         *reinterpret_cast<float4v*>(o.acc + 64 * c + 4 * n) =
-            float4v{st.acc[4 * c][i], st.acc[4 * c + 1][i], st.acc[4 * c + 2][i], st.acc[4 * c + 3][i]};
+            tile_out<DT, D>(st, c, i);
     }
   }
 }
