@@ -23,17 +23,22 @@ struct VarPlan {
   size_t ws_bytes = 0;
 };
 
-// Tokens of a sequence up to which one block takes them all (kOnePartitionFull where the
-// (sequence, kv head) pairs are about as many as the compute units), and the fewest that a
-// partition has otherwise.  Us, one block | partitions and a second launch that merges
-// them: 7 sequences x 8 kv heads of 240 tokens, Q8A, 64-wide 7.7 | 10.2; 48 x 4 of 700, f32
-// 16.8 | 21.5, f32 256-wide 54.7 | 84.0, f16 18.7 | 19.2, of 960 23.3 | 21.8; but 12 x 4 of
-// 440, f32 12.2 | 9.6, of 700 15.9 | 11.5.  Partitions of 64 | 128 | 192 | 256 | 512 tokens:
-// 24 x 4 of 1021, f32 16.6 | 15.3 | 17.5 | 15.8 | 19.5; 3 x 4 of 3700, Q8A 12.3 | 11.0 |
-// 10.9 | 11.6 | 16.2.
-constexpr int kOnePartition = 256;
+// Tokens of a sequence up to which one block takes them all, and the fewest that a
+// partition has otherwise (a second launch merges partitions).  kOnePartitionFull where the
+// (sequence, kv head) pairs are about as many as the compute units, else by what a page's
+// products cost.  Us, one block | partitions, 12 sequences x 4 kv heads of 8 heads: f16
+// 64-wide, 352 tokens 7.7 | 9.4, 480 8.5 | 9.9, 560 9.1 | 9.0; Q8A 352 9.0 | 9.7, 480 10.4 |
+// 9.6; f32 288 8.8 | 9.4, 352 10.0 | 9.5, 416 11.3 | 9.6; f32 128-wide, 2 x 8 of 288 11.7 |
+// 10.9, of 352 13.5 | 10.9; full, 48 x 4 of 700, f32 16.8 | 21.5, f32 256-wide 54.7 | 84.0,
+// f16 in f32 products 18.7 | 19.2, of 960 23.3 | 21.8.  Partitions of 64 | 128 | 192 | 256 |
+// 512 tokens: 24 x 4 of 1021, f32 16.6 | 15.3 | 17.5 | 15.8 | 19.5; 3 x 4 of 3700, Q8A 12.3 |
+// 11.0 | 10.9 | 11.6 | 16.2.
 constexpr int kOnePartitionFull = 768;
 constexpr int kLeastPartition = 128;
+inline int one_partition(const lnskv_pages* c, int n_seq) {
+  if ((int64_t)n_seq * c->n_kv_heads >= 192) return kOnePartitionFull;
+  return c->head_dim > 64 ? 256 : c->dtype == LNSKV_DTYPE_F16 ? 512 : 352;
+}
 
 inline bool var_mfma(const lnskv_pages* c) {
   return c->dtype != LNSKV_DTYPE_F32 && (c->head_dim == 128 || c->head_dim == 256);
@@ -43,9 +48,8 @@ inline bool var_mfma(const lnskv_pages* c) {
 // where those are few (a block's four waves share it and no merge is launched).
 inline int plan_tiles(const lnskv_pages* c, int n_seq, int n_heads, int64_t pages, VarPlan* p) {
   const int64_t tokens = std::max<int64_t>(pages, 1) * kPage;
-  const int64_t one = (int64_t)n_seq * c->n_kv_heads >= 192 ? kOnePartitionFull : kOnePartition;
   p->split = (int)tokens;
-  if (tokens > one)
+  if (tokens > one_partition(c, n_seq))
     p->split = std::max(kLeastPartition, choose_split(n_seq, (int)c->n_kv_heads, (int)std::min<int64_t>(tokens, INT32_MAX / 2)));
   const int64_t parts = (tokens + p->split - 1) / p->split;
   if (parts > 65535)

@@ -637,8 +637,8 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   const size_t row = ((size_t)d + 2) * sizeof(float);
   if (schedule_setting() == kScheduleAuto) {  // one launch for all pages
     const int64_t units = all * n_seq * c->n_kv_heads;
-    const int64_t bytes = units * kPage * 2 * d * (c->dtype == LNSKV_DTYPE_F16 ? 2 : 1);
-    if (var_mfma(c) ? all <= kDirectPages && bytes <= kDirectBytes : units * (d / 64) <= kDirectUnits * (7 + rep)) {
+    const int64_t page = kPage * 2 * d * (c->dtype == LNSKV_DTYPE_F16 ? 2 : 1);
+    if (var_mfma(c) ? all <= kDirectPages && units <= kDirectBytes / page : units * (d / 64) <= kDirectUnits * (7 + rep)) {
       p->direct = true;
       if (var_mfma(c)) return LNSKV_OK;
       if (int rc = plan_tiles(c, n_seq, n_heads, all, &p->own)) return rc;
