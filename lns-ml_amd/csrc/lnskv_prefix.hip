@@ -14,8 +14,7 @@
 //    a sequence with one share merges the prefix's rows and writes its output.
 // 3. join kernel, where sequences may have several shares: their rows and the
 //    prefix's into the output.
-// Small calls take one launch instead, in which each sequence reads its group's pages
-// itself (block kernel, or the tile kernel and its merge).
+// Small calls leave out step 1: each sequence reads its group's pages itself.
 #include "lnskv_decode_block.h"
 #include "lnskv_decode_var.h"
 #include "lnskv_prefill.h"
@@ -42,13 +41,16 @@ constexpr int kWidePages = 48;
 constexpr int kSharePages = 64;
 constexpr int kShareMin = 8;
 constexpr int kShareWhole = 32;
-// Small calls take one launch in which every sequence reads its group's pages itself, from
-// L2 mostly: on the matrix cores sequences of at most kDirectPages pages, kDirectBytes of K
-// and V in all, shared pages counted every time.  Us, one launch | prefix and own pages
-// apart, sequences x kv heads of pages: f16 128-wide 4 x 8 of 13 7.3 | 13.8, 16 x 8 of 57
-// 13.3 | 19.2, 64 x 8 of 57 (228 MB) 22.3 | 26.4, 128 x 8 of 57 (456 MB) 42.6 | 39.9, 16 x 8
-// of 107 20.8 | 21.2, 64 x 8 of 107 37 | 28.5; Q8A 128 x 8 of 57 (228 MB) 39.4 | 36.7,
-// 256-wide 64 x 4 of 26 17.4 | 26.6.
+// Small calls skip the prefix kernel: every sequence reads its group's pages itself, from
+// L2 mostly.  On the matrix cores sequences of at most kDirectPages pages (one share, one
+// launch), kDirectBytes of K and V in all with shared pages counted every time, and longer
+// ones of at most kDirectLong pages of 128 elements in all (shares and their join).  Us,
+// that | prefix and own pages apart, sequences x kv heads of pages: f16 128-wide 4 x 8 of 13
+// 7.3 | 13.8, 16 x 8 of 57 13.3 | 19.2, 64 x 8 of 57 (228 MB) 22.3 | 26.4, 128 x 8 of 57
+// (456 MB) 42.6 | 39.9; Q8A 128 x 8 of 57 (228 MB) 39.4 | 36.7, 256-wide 64 x 4 of 26 17.4 |
+// 26.6; longer, f16 128-wide 2 x 8 of 82 11.4 | 17.1, 5 x 8 of 163 15.3 | 22.1, 5 x 8 of 257
+// 22.2 | 20.2, 12 x 8 of 82 20.4 | 18.7, 12 x 4 of 82 19.2 | 25.4, 12 x 8 of 257 29.9 | 20.9;
+// Q8A 5 x 4 of 163 14.2 | 24.6, 256-wide 5 x 4 of 163 26.9 | 34.1, 12 x 4 of 257 47 | 34.
 // On the tile kernel kDirectUnits x (7 + heads per kv head) pages of 64 elements (a wave's
 // products cost the same for one head and for 16, so what the prefix kernel saves by tiles
 // of 16 rows falls with the heads): f32, 8 heads on one, 2 x 4 of 588 14 | 56, 6 x 4 of 588
@@ -57,6 +59,7 @@ constexpr int kShareWhole = 32;
 // 64-wide, 8 heads 6 x 4 of 588 19 | 36, 1 head 6 x 8 of 88 9.6 | 13.8.
 constexpr int kDirectPages = 64;
 constexpr int64_t kDirectBytes = (int64_t)192 << 20;
+constexpr int64_t kDirectLong = 10240;
 constexpr int64_t kDirectUnits = 1024;
 
 struct PrefixArgs {
@@ -423,7 +426,7 @@ __device__ __forceinline__ OwnSpan own_span(const DecodeArgs& a, const OwnArgs& 
   int L = a.kv_len[s];
   o.L = L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : max(L, 0);
   o.prefix = prefix_rows(x.prefix, s, a.n_heads);
-  o.p0 = min(o.prefix.pages * kPage, o.L);
+  o.p0 = x.prefix.split_pages > 0 ? min(o.prefix.pages * kPage, o.L) : 0;
   o.pages = o.L > o.p0 ? (o.L - 1) / kPage - o.p0 / kPage + 1 : 0;
   o.shares = max(1, ceil_div(o.pages, x.share_pages));
   return o;
@@ -463,6 +466,10 @@ void prefix_own_kernel(DecodeArgs a, OwnArgs x) {
   if (i0 < i1) {
     PieceLoads<REP, NH> pl;
     piece_loads<REP, false, false, Q8, NH>(a, s, kvh, o.p0 / kPage + i0, pl);
+    if (x.prefix.split_pages == 0) {  // shared pages too: fewer than the window's 64 entries a wave
+      const int e = i0 + lane;
+      if (e < a.bt_stride && e < o.prefix.pages) pl.btv = a.bt[(size_t)o.prefix.first * a.bt_stride + e];
+    }
     block_piece<REP, Q8, NH>(a, sm, wi, s, kvh, pl, o.p0 / kPage, i0, i1, o.L);
   }
   __syncthreads();
@@ -487,40 +494,6 @@ void prefix_own_kernel(DecodeArgs a, OwnArgs x) {
         x.own_ml[2 * r] = M;
         x.own_ml[2 * r + 1] = Ls;
       }
-    }
-  }
-}
-
-// Short sequences: a workgroup per (sequence, kv head) takes the shared pages and its own
-// in one launch.
-template <int REP, bool Q8, int NH>
-__global__ __launch_bounds__(kWave* kBlockWaves) __attribute__((amdgpu_waves_per_eu(NH == 1 ? 2 : 1)))
-void prefix_block_kernel(DecodeArgs a, VarArgs<kPrefix> x) {
-  constexpr int NW = kBlockWaves, D = NH * kD, C = D / kWave;
-  __shared__ BlockLds<REP, Q8, NH> sm;
-  const int wi = (int)(threadIdx.x / kWave), lane = (int)(threadIdx.x % kWave);
-  const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv), s = (int)(blockIdx.x / (unsigned)a.n_kv);
-  int L = a.kv_len[s];
-  L = L > min(a.max_kv_len, a.bt_stride * kPage) ? 0 : max(L, 0);
-  const PrefixRows pr = prefix_rows(x, s, a.n_heads);
-  const int np = (L + kPage - 1) / kPage, per = (np + NW - 1) / NW, i0 = min(np, wi * per), i1 = min(np, i0 + per);
-  if (i0 < i1) {
-    PieceLoads<REP, NH> pl;
-    piece_loads<REP, false, false, Q8, NH>(a, s, kvh, i0, pl);
-    const int e = i0 + lane;  // the wave's pages are fewer than the window's 64
-    if (e < a.bt_stride && e < pr.pages) pl.btv = a.bt[(size_t)pr.first * a.bt_stride + e];
-    block_piece<REP, Q8, NH>(a, sm, wi, s, kvh, pl, 0, i0, i1, L);
-  }
-  __syncthreads();
-  const int nw = np > 0 ? (np + per - 1) / per : 0;  // waves that left rows
-  for (int h = wi; h < REP; h += NW) {  // wave-uniform
-    float M, Ls, A[C];
-    block_merge<REP, Q8, NH>(sm, nw, h, M, Ls, A);
-    const size_t row = ((size_t)s * a.n_heads + (size_t)kvh * REP + h) * D;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const size_t i = row + c * kWave + lane;
-      a.out[i] = gated(a, i, Ls > 0.0f ? A[c] / Ls : 0.0f);
     }
   }
 }
@@ -559,16 +532,6 @@ void launch_own_rep(const DecodeArgs& a, const OwnArgs& x, int rep, unsigned blo
   }
 }
 
-template <bool Q8, int NH>
-void launch_block_rep(const DecodeArgs& a, const VarArgs<kPrefix>& x, int rep, unsigned blocks, hipStream_t st) {
-  switch (rep) {
-    case 1: prefix_block_kernel<1, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
-    case 2: prefix_block_kernel<2, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
-    case 4: prefix_block_kernel<4, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
-    default: prefix_block_kernel<8, Q8, NH><<<blocks, kWave * kBlockWaves, 0, st>>>(a, x); break;
-  }
-}
-
 template <bool Q8>
 void launch_prefix_mfma(const PrefixArgs& a, int d, int tile_rows, unsigned blocks, hipStream_t st) {
   if (d == 256)
@@ -592,7 +555,7 @@ void launch_prefix_tile(const PrefixArgs& a, int d, int64_t items, hipStream_t s
 // ---------------------------------------------------------------------------
 // The host's view of a call.
 struct PrefixPlan {
-  bool direct = false;    // one launch: every sequence reads the shared pages itself
+  bool direct = false;    // every sequence reads the shared pages itself
   VarPlan own;            // the tile kernel over the sequences' own pages
   int shares = 0;         // own kernel: shares of a sequence at most (0: the tile kernel)
   int share_pages = 0;
@@ -635,21 +598,21 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
   if (at < n_seq) most = all;
   own_pages += (n_seq - at) * all;
   const size_t row = ((size_t)d + 2) * sizeof(float);
-  if (schedule_setting() == kScheduleAuto) {  // one launch for all pages
+  if (schedule_setting() == kScheduleAuto) {
     const int64_t units = all * n_seq * c->n_kv_heads;
     const int64_t page = kPage * 2 * d * (c->dtype == LNSKV_DTYPE_F16 ? 2 : 1);
-    if (var_mfma(c) ? all <= kDirectPages && units <= kDirectBytes / page : units * (d / 64) <= kDirectUnits * (7 + rep)) {
-      p->direct = true;
-      if (var_mfma(c)) return LNSKV_OK;
-      if (int rc = plan_tiles(c, n_seq, n_heads, all, &p->own)) return rc;
-      p->ws_bytes = p->own.ws_bytes;
-      return LNSKV_OK;
+    p->direct = !var_mfma(c)           ? units * (d / 64) <= kDirectUnits * (7 + rep)
+                : all <= kDirectPages ? units <= kDirectBytes / page
+                                      : units * (d / 128) <= kDirectLong;
+    if (p->direct) {
+      own_pages = all * n_seq;
+      most = all;
     }
   }
   if (var_mfma(c)) {
     // shares of at most kSharePages pages, fewer where that leaves compute units idle
     const int64_t units = own_pages * c->n_kv_heads;
-    p->share_pages = n_seq * (int64_t)c->n_kv_heads >= 256 || most <= kShareWhole
+    p->share_pages = n_seq * (int64_t)c->n_kv_heads >= 256 || most <= (p->direct ? kDirectPages : kShareWhole)
                          ? kSharePages
                          : (int)std::min<int64_t>(kSharePages, std::max<int64_t>(kShareMin, (units + 511) / 512));
     p->shares = (int)std::max<int64_t>(1, (most + p->share_pages - 1) / p->share_pages);
@@ -661,7 +624,7 @@ int plan_prefix(const lnskv_pages* c, const int32_t* groups, int n_groups, int n
     if (int rc = plan_tiles(c, n_seq, n_heads, most, &p->own)) return rc;
     p->ws_bytes = p->own.ws_bytes;
   }
-  if (p->n_groups == 0) return LNSKV_OK;
+  if (p->n_groups == 0 || p->direct) return LNSKV_OK;
   // splits of equal pages: as many items as the card takes at once (a workgroup of
   // the matrix-core kernel per compute unit; of the tile kernel's waves two per SIMD
   // with 64-wide heads, else one)
@@ -730,18 +693,6 @@ int lnskv_prefix_decode(const lnskv_pages* c, const float* q, float* out, const 
   o.prefix.n_groups = p.n_groups;
   o.prefix.split_pages = p.direct ? 0 : p.split_pages;
   std::copy(p.g, p.g + p.n_groups, o.prefix.g);
-  if (p.direct && var_mfma(c)) {
-    const unsigned blocks = (unsigned)(n_seq * a.n_kv);
-    const int rep = n_heads / a.n_kv;
-    if (c->dtype == LNSKV_DTYPE_Q8A) {
-      if (d == 256) launch_block_rep<true, 2>(a, o.prefix, rep, blocks, st);
-      else launch_block_rep<true, 1>(a, o.prefix, rep, blocks, st);
-    } else {
-      if (d == 256) launch_block_rep<false, 2>(a, o.prefix, rep, blocks, st);
-      else launch_block_rep<false, 1>(a, o.prefix, rep, blocks, st);
-    }
-    return hip_check("decode kernel launch");
-  }
   if (p.n_groups > 0 && !p.direct) {
     PrefixArgs x{};
     x.pf.k_pages = a.k_pages;
